@@ -36,7 +36,7 @@ extern "C" {
 #define UGK_ST_PLACE_PROMISE 0x20u   /* ugk_rank_place_observed: k or more rows were observed; nothing was placed */
 #define UGK_ST_SLOT_CLASH 0x40u      /* ugk_handed_check, ugk_table_insert_handed_*: a cache slot listed twice, or one not in use */
 
-/* element code of the pooled extraction for bfloat16 rows (fp32 and fp16 are named by their size, 4 and 2) */
+/* element code of bfloat16 rows (fp32 and fp16 are named by their size, 4 and 2) */
 #define UGK_ELEM_BF16 0x102
 
 /* ---- locations (cache_context.cu:2421-2422: GPUs are 0..G-1, the host is G; here G = 1) ---------- */
@@ -104,7 +104,7 @@ typedef struct {
 const char *ugk_last_error(void);
 /* version of this ABI; bumped on any signature change.  ugk_abi_version() is what the loaded library was built with:
  * a caller compiled against another UGK_ABI_VERSION must not go on. */
-#define UGK_ABI_VERSION 27
+#define UGK_ABI_VERSION 28
 int ugk_abi_version(void);
 
 /* ---- runtime plumbing: Device::{AllocDataSpace,FreeDataSpace,CopyDataFromTo,StreamSync,CreateStream}
@@ -467,6 +467,76 @@ int ugk_gather_scatter_staged_u32(const void *host_dev, uint64_t host_rows, cons
                                   size_t row_bytes, ugk_stage_t stage, unsigned max_blocks, uint32_t *status_dev,
                                   uint32_t *staged_dev, uint32_t *rest_rows_dev, uint32_t *rest_dst_off_dev,
                                   uint32_t *rest_count_dev, uint32_t *done_count_dev, void *stream);
+
+/* ---- rows sent to a router's experts and back (no counterpart in the reference) --------------------------------------
+ * A router names `top` of num_experts experts for every token.  ids_dev[t * top + k] is the k-th expert of token t; an id
+ * outside [0, num_experts) is an assignment without one (padding, an expert of another GPU).  ugk_expert_sort_* puts the n =
+ * tokens * top assignments in order of their experts, within an expert in order of the assignments:
+ *   offsets_dev[e] .. offsets_dev[e + 1]   the positions of expert e (num_experts + 1 words; the last one is the number of
+ *                                          live assignments)
+ *   slot_dev[i]                            the position of assignment i, -1 without an expert
+ *   src_dev[p]                             the assignment at position p, -1 behind the last one
+ * num_experts: 1 to 1024; n < 2^31.  The same ids give the same order on every run. */
+size_t ugk_expert_sort_workspace_bytes(size_t n, uint32_t num_experts);
+int ugk_expert_sort_i32(const int32_t *ids_dev, size_t n, uint32_t num_experts, int32_t *slot_dev, int32_t *src_dev,
+                        int32_t *offsets_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+int ugk_expert_sort_i64(const int64_t *ids_dev, size_t n, uint32_t num_experts, int32_t *slot_dev, int32_t *src_dev,
+                        int32_t *offsets_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+/* Rows are `dim` elements of code elem (4 = fp32, 2 = fp16, UGK_ELEM_BF16), `stride` elements apart where a stride is
+ * given and dense elsewhere, at any element's address; live_dev = offsets_dev + num_experts.
+ *
+ * dispatch:      rows[slot[t, k]] = x[t]; the rows from *live_dev to tokens * top are zero.
+ * combine:       out[t] = sum over k of w[t, k] * rows[slot[t, k]]; weights_dev NULL: w = 1, which is the gradient of the
+ *                dispatch.  Added in fp32 in the order of k, rounded once; an assignment without a position adds nothing.
+ * combine_grad:  grad_rows[slot[t, k]] = w[t, k] * grad_out[t], the rows from *live_dev on zero;
+ *                grad_weights[t, k] = <rows[slot[t, k]], grad_out[t]> in fp32, zero without a position (grad_weights_dev
+ *                NULL: not wanted, and rows_dev is not read).
+ * The weights and their gradient are of code weight_elem.  A position beyond the rows is treated as none; two assignments
+ * at one position, which ugk_expert_sort_* never makes, leave one of the two rows there. */
+int ugk_expert_dispatch(const void *x_dev, size_t x_stride, const int32_t *slot_dev, const int32_t *live_dev, size_t tokens,
+                        uint32_t top, size_t dim, int elem, void *rows_dev, void *stream);
+int ugk_expert_combine(const void *rows_dev, size_t n_rows, size_t row_stride, const int32_t *slot_dev, size_t tokens,
+                       uint32_t top, const void *weights_dev, int weight_elem, size_t dim, int elem, void *out_dev, void *stream);
+int ugk_expert_combine_grad(const void *grad_out_dev, size_t grad_stride, const void *rows_dev, size_t row_stride,
+                            const int32_t *slot_dev, const int32_t *live_dev, size_t tokens, uint32_t top,
+                            const void *weights_dev, int weight_elem, size_t dim, int elem, void *grad_rows_dev,
+                            void *grad_weights_dev, void *stream);
+
+/* ---- rows that are trained -------------------------------------------------------------------------------------------
+ * take_rows:       out[i] = table[index[i]], bit for bit; an index outside [0, num_rows) gives a zero row (padding) and is no
+ *                  error, unlike a key of ugk_gather_direct_*.
+ * take_rows_grad:  out[r] = sum of grad[i] over all i with index[i] = r, in fp32, rounded once; a row without an entry is
+ *                  zero, entries outside [0, num_rows) add nothing.  What training a table asks for behind
+ *                  ugk_gather_direct_* (index = key), and behind ugk_dedup_* (index = inverse: the gradient of the distinct
+ *                  rows).  The order of additions follows from the index alone: no two runs differ.  n, num_rows < 2^31.
+ * Sizes, strides and element codes as above; the workspace is the caller's. */
+int ugk_take_rows_i32(const void *table_dev, uint64_t num_rows, size_t stride, const int32_t *index_dev, size_t n, size_t dim,
+                      int elem, void *out_dev, void *stream);
+int ugk_take_rows_i64(const void *table_dev, uint64_t num_rows, size_t stride, const int64_t *index_dev, size_t n, size_t dim,
+                      int elem, void *out_dev, void *stream);
+size_t ugk_take_rows_grad_workspace_bytes(size_t n, uint64_t num_rows);
+int ugk_take_rows_grad_i32(const void *grad_dev, size_t stride, const int32_t *index_dev, size_t n, uint64_t num_rows, size_t dim,
+                           int elem, void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+int ugk_take_rows_grad_i64(const void *grad_dev, size_t stride, const int64_t *index_dev, size_t n, uint64_t num_rows, size_t dim,
+                           int elem, void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* A gradient of ugk_grad_*: `count` dense elements of code elem at any element's address.  The list is host memory and is
+ * read before the call returns. */
+typedef struct {
+  const void *data; /* device; written by ugk_grad_clip where out is NULL */
+  void *out;        /* where ugk_grad_clip puts the scaled elements; NULL: in place */
+  uint64_t count;
+  int32_t elem;
+  int32_t reserved;
+} ugk_tensor_t;
+/* norm:  *norm_dev = sqrt of the sum of the squares of all elements of all tensors, squares and sums held in 64 bits.
+ * clip:  the norm, and every element multiplied by min(1, max_norm / (norm + 1e-6)), rounded once.  A norm that is no number
+ *        makes every element none; an infinite one makes the finite elements zero.
+ * The tensors do not overlap one another's outputs.  The same gradients give the same bits on every run. */
+size_t ugk_grad_norm_workspace_bytes(const ugk_tensor_t *tensors, size_t n);
+int ugk_grad_norm(const ugk_tensor_t *tensors, size_t n, void *workspace_dev, size_t workspace_bytes, float *norm_dev, void *stream);
+int ugk_grad_clip(const ugk_tensor_t *tensors, size_t n, double max_norm, void *workspace_dev, size_t workspace_bytes,
+                  float *norm_dev, void *stream);
 
 /* ---- key dedup (the caller-side array_ops.unique of
  *      python_tf2/collcache_tf2/collcache_tf2/core/sparse_lookup_layer.py:197) ------------------------

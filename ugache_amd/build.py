@@ -24,7 +24,7 @@ HIP_LIB = os.path.join(PKG, "libugache_hip.so")
 HOST_LIB = os.path.join(PKG, "libcoll_cache.so")
 
 HIP_SOURCES = ["ugk_partition.hip", "ugk_pool_i64.hip", "ugk_pool.hip", "ugk_gather.hip", "ugk_refresh.hip",
-               "ugk_runtime.hip", "ugk_table.hip", "ugk_hotness.hip"]
+               "ugk_runtime.hip", "ugk_table.hip", "ugk_hotness.hip", "ugk_expert.hip", "ugk_take_rows.hip", "ugk_grad_norm.hip"]
 OBJ_DIR = os.path.join(PKG, "_build")
 
 HIPCC_FLAGS = [

@@ -2,7 +2,7 @@
 `collcache.torch`, each a thin forwarder into the binding module `collcache.torch.c_lib` (adapter.py:25-60)."""
 from ..common import *  # noqa: F401,F403
 from ..common import _basics
-from . import c_lib
+from . import c_lib, rows
 
 config = _basics.config
 log_step_by_key = _basics.log_step_by_key
@@ -49,3 +49,15 @@ coll_torch_forward_join = c_lib.coll_torch_forward_join
 coll_torch_load_raw_model = c_lib.coll_torch_load_raw_model
 coll_torch_refresh = c_lib.coll_torch_refresh
 coll_torch_shutdown = c_lib.coll_torch_shutdown
+
+# rows that go to experts and back, rows that are trained, the norm over gradients
+ExpertOrder = rows.ExpertOrder
+coll_torch_expert_sort = rows.coll_torch_expert_sort
+coll_torch_expert_dispatch = rows.coll_torch_expert_dispatch
+coll_torch_expert_dispatch_grad = rows.coll_torch_expert_dispatch_grad
+coll_torch_expert_combine = rows.coll_torch_expert_combine
+coll_torch_expert_combine_grad = rows.coll_torch_expert_combine_grad
+coll_torch_take_rows = rows.coll_torch_take_rows
+coll_torch_take_rows_grad = rows.coll_torch_take_rows_grad
+coll_torch_grad_norm = rows.coll_torch_grad_norm
+coll_torch_clip_grad_norm = rows.coll_torch_clip_grad_norm

@@ -1,0 +1,106 @@
+// Rows of fp32, fp16 or bfloat16 elements of any length at any element boundary, as the kernels that add, weight and
+// move them see them: 16-byte chunks held in registers as floats.
+//
+// A row of at least one chunk is covered by chunks at multiples of a chunk's length, the last one moved back so that it ends
+// with the row: elements that two chunks share are computed twice, to the same bits, and no lane needs a loop over a
+// tail.  gfx950 loads and stores 16 bytes at any element's address, so an odd number of two-byte elements costs no
+// kernel of its own.  Rows shorter than a chunk go element by element (VEC 1).
+#pragma once
+
+#include <type_traits>
+
+#include "ugk_internal.h"
+
+namespace ugk {
+namespace {
+
+// the element types: how they are stored, and converted (to float exactly, back to the nearest, ties to even)
+typedef _Float16 half_t;
+typedef __bf16 bhalf_t;
+
+template <typename T, int VEC>
+struct ChunkOf {
+  typedef T type __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+};
+template <typename T>
+struct ChunkOf<T, 1> {
+  typedef T type;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_chunk(const T *from, float (&x)[VEC]) {
+  const typename ChunkOf<T, VEC>::type v = *reinterpret_cast<const typename ChunkOf<T, VEC>::type *>(from);
+  if constexpr (VEC == 1) {
+    x[0] = (float)v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = (float)v[i];
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_chunk(T *to, const float (&x)[VEC]) {
+  typename ChunkOf<T, VEC>::type v;
+  if constexpr (VEC == 1) {
+    v = (T)x[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = (T)x[i];
+  }
+  *reinterpret_cast<typename ChunkOf<T, VEC>::type *>(to) = v;
+}
+
+// a weight of any of the three types (a branch that the whole launch takes the same way)
+__device__ __forceinline__ float load_weight(const void *w, int elem, size_t i) {
+  if (elem == 4) return static_cast<const float *>(w)[i];
+  if (elem == 2) return (float)static_cast<const half_t *>(w)[i];
+  return (float)static_cast<const bhalf_t *>(w)[i];
+}
+__device__ __forceinline__ void store_weight(void *w, int elem, size_t i, float v) {
+  if (elem == 4) static_cast<float *>(w)[i] = v;
+  else if (elem == 2) static_cast<half_t *>(w)[i] = (half_t)v;
+  else static_cast<bhalf_t *>(w)[i] = (bhalf_t)v;
+}
+
+// How the chunks of a batch of rows are dealt to lanes: numbered through, so that no lane idles whatever a row's length.
+struct Split {
+  uint32_t chunks;  // of a row
+  uint32_t magic;   // floor(2^32 / chunks) + 1, where that has 32 bits
+};
+static inline Split split_of(size_t dim, int vec) {
+  const uint32_t chunks = (uint32_t)((dim + vec - 1) / vec);
+  return Split{chunks, (uint32_t)(((uint64_t)1 << 32) / chunks + 1)};
+}
+static inline size_t split_blocks(size_t rows, const Split &s) { return (rows * s.chunks + kBlock - 1) / kBlock; }
+
+// the row and the chunk of a lane.  The division of the workgroup's first number is scalar; what a lane adds to its remainder
+// stays below chunks + 256, where the product with the magic number is exact for up to 256 chunks and a comparison does
+// for more.
+__device__ __forceinline__ void split_lane(const Split &s, size_t &row, uint32_t &chunk) {
+  const uint64_t first = (uint64_t)blockIdx.x * kBlock;
+  const uint64_t row0 = first / s.chunks;
+  const uint32_t at = (uint32_t)(first - row0 * s.chunks) + threadIdx.x;
+  const uint32_t over = s.chunks == 1 ? at : s.chunks > (uint32_t)kBlock ? (at >= s.chunks ? 1u : 0u) : __umulhi(at, s.magic);
+  row = row0 + over;
+  chunk = at - over * s.chunks;
+}
+
+// calls f with the element type and the elements per chunk that rows of `dim` elements of code `elem` take
+template <typename F>
+static inline int for_rows(int elem, size_t dim, F f) {
+  if (elem == 4) return dim >= 4 ? f(float(), std::integral_constant<int, 4>()) : f(float(), std::integral_constant<int, 1>());
+  if (elem == 2) return dim >= 8 ? f(half_t(), std::integral_constant<int, 8>()) : f(half_t(), std::integral_constant<int, 1>());
+  return dim >= 8 ? f(bhalf_t(), std::integral_constant<int, 8>()) : f(bhalf_t(), std::integral_constant<int, 1>());
+}
+// ... for kernels that move elements of two or four bytes without looking at them
+template <typename F>
+static inline int for_moved_rows(int elem, size_t dim, F f) {
+  if (elem == 4) return dim >= 4 ? f(uint32_t(), std::integral_constant<int, 4>()) : f(uint32_t(), std::integral_constant<int, 1>());
+  return dim >= 8 ? f(uint16_t(), std::integral_constant<int, 8>()) : f(uint16_t(), std::integral_constant<int, 1>());
+}
+
+static inline bool elem_ok(int elem) { return elem == 4 || elem == 2 || elem == UGK_ELEM_BF16; }
+static inline size_t elem_size(int elem) { return elem == 4 ? 4 : 2; }
+
+}  // namespace
+}  // namespace ugk

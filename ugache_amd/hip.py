@@ -152,6 +152,20 @@ SIGNATURES = {
     "ugk_extract_mix_staged_i64": [Table, _vp, _sz, _vp, _u64, _vp, _u64, _vp, _sz, _vp, _vp, _vp, _vp, _u32, Stage, _vp],
     "ugk_gather_scatter_staged_u32": [_vp, _u64, _vp, _vp, _sz, _vp, _u64, _sz, Stage, C.c_uint, _vp, _vp, _vp, _vp,
                                       _vp, _vp, _vp],
+    "ugk_expert_sort_workspace_bytes": [_sz, _u32],
+    "ugk_expert_sort_i32": [_vp, _sz, _u32, _vp, _vp, _vp, _vp, _sz, _vp],
+    "ugk_expert_sort_i64": [_vp, _sz, _u32, _vp, _vp, _vp, _vp, _sz, _vp],
+    "ugk_expert_dispatch": [_vp, _sz, _vp, _vp, _sz, _u32, _sz, C.c_int, _vp, _vp],
+    "ugk_expert_combine": [_vp, _sz, _sz, _vp, _sz, _u32, _vp, C.c_int, _sz, C.c_int, _vp, _vp],
+    "ugk_expert_combine_grad": [_vp, _sz, _vp, _sz, _vp, _vp, _sz, _u32, _vp, C.c_int, _sz, C.c_int, _vp, _vp, _vp],
+    "ugk_take_rows_i32": [_vp, _u64, _sz, _vp, _sz, _sz, C.c_int, _vp, _vp],
+    "ugk_take_rows_i64": [_vp, _u64, _sz, _vp, _sz, _sz, C.c_int, _vp, _vp],
+    "ugk_take_rows_grad_workspace_bytes": [_sz, _u64],
+    "ugk_take_rows_grad_i32": [_vp, _sz, _vp, _sz, _u64, _sz, C.c_int, _vp, _vp, _sz, _vp],
+    "ugk_take_rows_grad_i64": [_vp, _sz, _vp, _sz, _u64, _sz, C.c_int, _vp, _vp, _sz, _vp],
+    "ugk_grad_norm_workspace_bytes": [_vp, _sz],
+    "ugk_grad_norm": [_vp, _sz, _vp, _sz, _vp, _vp],
+    "ugk_grad_clip": [_vp, _sz, C.c_double, _vp, _sz, _vp, _vp],
     "ugk_dedup_workspace_bytes": [_sz],
     "ugk_dedup_u32": [_vp, _sz, _vp, _sz, _u32, _vp, _vp, _vp, _vp, _vp, _vp],
     "ugk_dedup_i64": [_vp, _sz, _vp, _sz, _u32, _vp, _vp, _vp, _vp, _vp, _vp],
@@ -179,6 +193,7 @@ SIGNATURES = {
     "ugk_last_error": [],
 }
 _RESTYPES = {"ugk_extract_mix_max_groups": C.c_uint, "ugk_hash_buckets_for": _sz, "ugk_hash32_entries_for": _sz, "ugk_dedup_workspace_bytes": _sz, "ugk_rank_workspace_bytes": _sz,
+             "ugk_expert_sort_workspace_bytes": _sz, "ugk_take_rows_grad_workspace_bytes": _sz, "ugk_grad_norm_workspace_bytes": _sz,
              "ugk_bitmap_workspace_bytes": _sz, "ugk_last_error": C.c_char_p}
 _NO_CHECK = set(_RESTYPES) | {"ugk_abi_version"}
 
