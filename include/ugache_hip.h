@@ -514,7 +514,7 @@ int ugk_take_rows_i32(const void *table_dev, uint64_t num_rows, size_t stride, c
                       int elem, void *out_dev, void *stream);
 int ugk_take_rows_i64(const void *table_dev, uint64_t num_rows, size_t stride, const int64_t *index_dev, size_t n, size_t dim,
                       int elem, void *out_dev, void *stream);
-size_t ugk_take_rows_grad_workspace_bytes(size_t n, uint64_t num_rows);
+size_t ugk_take_rows_grad_workspace_bytes(size_t n, uint64_t num_rows, size_t dim);
 int ugk_take_rows_grad_i32(const void *grad_dev, size_t stride, const int32_t *index_dev, size_t n, uint64_t num_rows, size_t dim,
                            int elem, void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
 int ugk_take_rows_grad_i64(const void *grad_dev, size_t stride, const int64_t *index_dev, size_t n, uint64_t num_rows, size_t dim,

@@ -283,7 +283,7 @@ def coll_torch_take_rows_grad(grad, index, num_rows):
     if not 0 <= num_rows < 1 << 31 or n >= 1 << 31:
         raise ValueError("%d indices into %d rows: both must be below 2^31" % (n, num_rows))
     out = torch.empty(num_rows, g.size(1), dtype=g.dtype, device=g.device)
-    nbytes = _L.ugk_take_rows_grad_workspace_bytes(n, num_rows)
+    nbytes = _L.ugk_take_rows_grad_workspace_bytes(n, num_rows, g.size(1))
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=g.device)
     _launch(_L.ugk_take_rows_grad_i64 if flat.dtype == torch.int64 else _L.ugk_take_rows_grad_i32, dev, g.data_ptr(), stride,
             flat.data_ptr(), n, num_rows, g.size(1), _ELEM[g.dtype], out.data_ptr(), workspace.data_ptr(), nbytes)

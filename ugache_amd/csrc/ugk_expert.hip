@@ -18,7 +18,7 @@ __global__ __launch_bounds__(kBlock) void dispatch_kernel(const T *__restrict__ 
   typedef typename ChunkOf<T, VEC>::type chunk_t;
   size_t t;
   uint32_t c;
-  split_lane(split, t, c);
+  split_lane(split, blockIdx.x, t, c);
   if (t >= tokens) return;
   const uint32_t at = min(c * VEC, dim - VEC);
   const chunk_t v = *reinterpret_cast<const chunk_t *>(x + t * x_stride + at);
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kBlock) void combine_kernel(const T *__restrict__ r
                                                          Split split, T *__restrict__ out) {
   size_t t;
   uint32_t c;
-  split_lane(split, t, c);
+  split_lane(split, blockIdx.x, t, c);
   if (t >= tokens) return;
   const uint32_t at = min(c * VEC, dim - VEC);
   float sum[VEC] = {};

@@ -76,8 +76,8 @@ static inline size_t split_blocks(size_t rows, const Split &s) { return (rows * 
 // the row and the chunk of a lane.  The division of the workgroup's first number is scalar; what a lane adds to its remainder
 // stays below chunks + 256, where the product with the magic number is exact for up to 256 chunks and a comparison does
 // for more.
-__device__ __forceinline__ void split_lane(const Split &s, size_t &row, uint32_t &chunk) {
-  const uint64_t first = (uint64_t)blockIdx.x * kBlock;
+__device__ __forceinline__ void split_lane(const Split &s, uint32_t block, size_t &row, uint32_t &chunk) {
+  const uint64_t first = (uint64_t)block * kBlock;
   const uint64_t row0 = first / s.chunks;
   const uint32_t at = (uint32_t)(first - row0 * s.chunks) + threadIdx.x;
   const uint32_t over = s.chunks == 1 ? at : s.chunks > (uint32_t)kBlock ? (at >= s.chunks ? 1u : 0u) : __umulhi(at, s.magic);

@@ -1,8 +1,8 @@
 // Rows taken by index, and the gradient of that: the rows of equal indices added up.
 //
-// The gradient sorts the entries by the row they name (digits of up to ten bits, ugk_bucket_sort.cuh), finds where
-// every row's entries begin, and adds them in fp32 in the order of the batch: no atomic touches a sum, so the same
-// batch gives the same bits on every run.
+// The gradient sorts the entries by the row they name (digits of up to ten bits, ugk_bucket_sort.cuh), finds where every row's
+// entries begin, and adds them in fp32 in the order of the batch, those of a row that many entries name in pieces that are
+// then added in their order: no atomic touches a sum, so the same batch gives the same bits on every run.
 #include <type_traits>
 
 #include "ugk_bucket_sort.cuh"
@@ -18,7 +18,7 @@ __global__ __launch_bounds__(kBlock) void take_rows_kernel(const T *__restrict__
   typedef typename ChunkOf<T, VEC>::type chunk_t;
   size_t i;
   uint32_t c;
-  split_lane(split, i, c);
+  split_lane(split, blockIdx.x, i, c);
   if (i >= n) return;
   const uint32_t at = min(c * VEC, dim - VEC);
   const long long r = (long long)index[i];
@@ -27,34 +27,122 @@ __global__ __launch_bounds__(kBlock) void take_rows_kernel(const T *__restrict__
   *reinterpret_cast<chunk_t *>(out + i * dim + at) = v;
 }
 
-// begin[r] = number of sorted keys below r, r = 0 .. rows: lane i writes the rows that begin between entry i - 1 and entry i
-__global__ __launch_bounds__(kBlock) void row_begin_kernel(const uint32_t *__restrict__ keys, size_t n, uint32_t rows,
+// begin[r] = number of sorted keys below r, r = 0 .. rows.  A search per row, so that neither a run of rows nobody named nor a
+// row everybody named is one lane's work; neighbouring rows walk the same way, a request for a wavefront.
+__global__ __launch_bounds__(kBlock) void row_begin_kernel(const uint32_t *__restrict__ keys, uint32_t n, uint32_t rows,
                                                            uint32_t *__restrict__ begin) {
-  const size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i > n) return;
-  const uint32_t from = i == 0 ? 0u : keys[i - 1] + 1u, to = i == n ? rows : min(keys[i], rows);
-  for (uint32_t r = from; r <= to; ++r) begin[r] = (uint32_t)i;
+  const uint32_t r = blockIdx.x * kBlock + threadIdx.x;
+  if (r > rows) return;
+  uint32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (keys[mid] < r) lo = mid + 1;
+    else hi = mid;
+  }
+  begin[r] = lo;
 }
 
-// out[r] = sum of the rows grad[entries[j]], begin[r] <= j < begin[r + 1], in fp32 in the order of j
+// sum += the rows grad[entries[j]], from <= j < to, in the order of j
 template <typename T, int VEC>
-__global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ grad, size_t stride, const uint32_t *__restrict__ entries,
-                                                         const uint32_t *__restrict__ begin, size_t rows, uint32_t dim, Split split,
-                                                         T *__restrict__ out) {
-  size_t r;
-  uint32_t c;
-  split_lane(split, r, c);
-  if (r >= rows) return;
-  const uint32_t at = min(c * VEC, dim - VEC);
-  float sum[VEC] = {};
-  const uint32_t end = begin[r + 1];
-  for (uint32_t j = begin[r]; j < end; ++j) {
+__device__ __forceinline__ void add_entries(const T *grad, size_t stride, const uint32_t *entries, uint32_t from, uint32_t to, uint32_t at,
+                                            float (&sum)[VEC]) {
+  constexpr int U = 4;  // rows on their way
+  uint32_t j = from;
+  for (; j + U <= to; j += U) {
+    float v[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_chunk<T, VEC>(grad + (size_t)entries[j + u] * stride + at, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] += v[u][e];
+  }
+  for (; j < to; ++j) {
     float v[VEC];
     load_chunk<T, VEC>(grad + (size_t)entries[j] * stride + at, v);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[e] += v[e];
   }
-  store_chunk<T, VEC>(out + r * dim + at, sum);
+}
+
+// A row of more than kPiece entries is summed in pieces: the positions are cut into pieces of kPiece, and a piece holds parts
+// of at most two such rows, one that comes in from the piece before and one that begins in it and goes on behind it.
+// parts[2 * piece] and parts[2 * piece + 1] are their sums.
+constexpr uint32_t kPiece = 64;
+
+// out[r] = sum of the rows grad[entries[j]], begin[r] <= j < begin[r + 1], in fp32 in the order of j.  The first row_blocks
+// workgroups take the rows of at most kPiece entries, the others the pieces.
+template <typename T, int VEC>
+__global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ grad, size_t stride, const uint32_t *__restrict__ entries,
+                                                         const uint32_t *__restrict__ keys, const uint32_t *__restrict__ begin,
+                                                         uint32_t rows, uint32_t dim, Split split, uint32_t row_blocks, T *__restrict__ out,
+                                                         float *__restrict__ parts) {
+  size_t i;
+  uint32_t c;
+  const bool whole = blockIdx.x < row_blocks;
+  split_lane(split, whole ? blockIdx.x : blockIdx.x - row_blocks, i, c);
+  const uint32_t at = min(c * VEC, dim - VEC);
+  float sum[VEC] = {};
+  if (whole) {
+    if (i >= rows) return;
+    const uint32_t from = begin[i], to = begin[i + 1];
+    if (to - from > kPiece) return;
+    add_entries<T, VEC>(grad, stride, entries, from, to, at, sum);
+    store_chunk<T, VEC>(out + i * dim + at, sum);
+    return;
+  }
+  const uint32_t live = begin[rows];
+  const uint64_t first = i * kPiece;
+  if (first >= live) return;
+  const uint32_t from = (uint32_t)first, to = (uint32_t)min(first + kPiece, (uint64_t)live);
+  const uint32_t r0 = keys[from], begin0 = begin[r0], end0 = begin[r0 + 1];
+  if (begin0 < from && end0 - begin0 > kPiece) {
+    add_entries<T, VEC>(grad, stride, entries, from, min(to, end0), at, sum);
+    store_chunk<float, VEC>(parts + 2 * i * dim + at, sum);
+  }
+  const uint32_t r1 = keys[to - 1], begin1 = begin[r1];
+  if (begin1 >= from && begin[r1 + 1] - begin1 > kPiece) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
+    add_entries<T, VEC>(grad, stride, entries, begin1, to, at, sum);
+    store_chunk<float, VEC>(parts + (2 * i + 1) * dim + at, sum);
+  }
+}
+
+// The pieces of a row added up: a workgroup per piece in which such a row begins and per `lanes` chunks of it.  kBlock /
+// lanes groups of lanes add a run of the pieces each, then the groups' sums are added in their order.
+template <typename T, int VEC>
+__global__ __launch_bounds__(kBlock) void row_join_kernel(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ begin, uint32_t rows,
+                                                          uint32_t dim, uint32_t chunks, uint32_t lanes, const float *__restrict__ parts,
+                                                          T *__restrict__ out) {
+  __shared__ float held[kBlock * VEC];
+  const uint32_t live = begin[rows];
+  const uint64_t first = (uint64_t)blockIdx.x * kPiece;
+  if (first >= live) return;
+  const uint32_t r = keys[min(first + kPiece, (uint64_t)live) - 1], from = begin[r], to = begin[r + 1];
+  if (from < first || to - from <= kPiece) return;
+  const uint32_t group = threadIdx.x / lanes, groups = kBlock / lanes;  // lanes: a power of two
+  const uint32_t c = blockIdx.y * lanes + threadIdx.x % lanes;
+  const uint32_t at = min(c * VEC, dim - VEC);
+  const uint32_t p0 = blockIdx.x, pieces = (to - 1) / kPiece - p0 + 1;
+  const uint32_t per = (pieces + groups - 1) / groups;
+  float sum[VEC] = {};
+  if (c < chunks) {
+    for (uint32_t p = group * per; p < min((group + 1) * per, pieces); ++p) {
+      float v[VEC];
+      load_chunk<float, VEC>(parts + (2 * (size_t)(p0 + p) + (p == 0 ? 1 : 0)) * dim + at, v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] += v[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) held[e * kBlock + threadIdx.x] = sum[e];
+  __syncthreads();
+  if (group != 0 || c >= chunks) return;
+  for (uint32_t g = 1; g < groups; ++g)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum[e] += held[e * kBlock + g * lanes + threadIdx.x];
+  store_chunk<T, VEC>(out + (size_t)r * dim + at, sum);
 }
 
 __global__ void preload_take_rows_kernel() {}
@@ -94,6 +182,8 @@ Plan plan_for(uint64_t rows) {
   return Plan{passes, (bits + passes - 1) / passes};
 }
 
+size_t pieces_of(size_t n) { return (n + kPiece - 1) / kPiece; }
+
 template <typename I>
 int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, uint64_t num_rows, size_t dim, int elem, void *out,
                    void *workspace, size_t workspace_bytes, void *stream) {
@@ -104,11 +194,12 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
   UGK_REQUIRE(stride >= dim || n <= 1, "ugk_take_rows_grad: rows of %zu elements overlap at a stride of %zu", dim, stride);
   if (num_rows == 0) return 0;
   UGK_REQUIRE(out && (n == 0 || (grad && index)), "ugk_take_rows_grad: null pointer");
-  const size_t need = ugk_take_rows_grad_workspace_bytes(n, num_rows);
+  const size_t need = ugk_take_rows_grad_workspace_bytes(n, num_rows, dim);
   UGK_REQUIRE(workspace && workspace_bytes >= need, "ugk_take_rows_grad: a workspace of %zu bytes, %zu are needed", workspace_bytes, need);
   uint32_t *begin = static_cast<uint32_t *>(workspace);
   uint32_t *key[2] = {begin + num_rows + 1, begin + num_rows + 1 + n}, *entry[2] = {key[1] + n, key[1] + 2 * n};
-  uint32_t *words = entry[1] + n;
+  float *parts = reinterpret_cast<float *>(entry[1] + n);
+  uint32_t *words = reinterpret_cast<uint32_t *>(parts + 2 * pieces_of(n) * dim);
   const Plan p = plan_for(num_rows);
   int at = 0;
   if (n > 0) {
@@ -120,16 +211,21 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
         return rc;
     }
   }
-  hipLaunchKernelGGL(row_begin_kernel, dim3((unsigned)(n / kBlock + 1)), dim3(kBlock), 0, as_stream(stream), key[at], n, (uint32_t)num_rows,
-                     begin);
+  hipLaunchKernelGGL(row_begin_kernel, dim3((unsigned)(num_rows / kBlock + 1)), dim3(kBlock), 0, as_stream(stream), key[at], (uint32_t)n,
+                     (uint32_t)num_rows, begin);
   return for_rows(elem, dim, [&](auto type, auto vec) -> int {
     typedef decltype(type) T;
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
-    const size_t blocks = split_blocks(num_rows, s);
-    UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_take_rows_grad: %zu rows of %zu elements are more than one launch takes", (size_t)num_rows, dim);
+    const size_t pieces = n > kPiece ? pieces_of(n) : 0;  // in fewer entries no row has more than a piece
+    const size_t row_blocks = split_blocks(num_rows, s), blocks = row_blocks + split_blocks(pieces, s);
+    uint32_t lanes = 1;
+    while (lanes < s.chunks && lanes < 32) lanes *= 2;
     hipLaunchKernelGGL((row_sum_kernel<T, V>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)grad, stride, entry[at],
-                       begin, num_rows, (uint32_t)dim, s, (T *)out);
+                       key[at], begin, (uint32_t)num_rows, (uint32_t)dim, s, (uint32_t)row_blocks, (T *)out, parts);
+    if (pieces > 0)
+      hipLaunchKernelGGL((row_join_kernel<T, V>), dim3((unsigned)pieces, (s.chunks + lanes - 1) / lanes), dim3(kBlock), 0, as_stream(stream),
+                         key[at], begin, (uint32_t)num_rows, (uint32_t)dim, s.chunks, lanes, parts, (T *)out);
     UGK_HIP(hipGetLastError());
     return 0;
   });
@@ -151,8 +247,8 @@ int ugk_take_rows_i64(const void *table_dev, uint64_t num_rows, size_t stride, c
   return take_rows<int64_t>(table_dev, num_rows, stride, index_dev, n, dim, elem, out_dev, stream);
 }
 
-size_t ugk_take_rows_grad_workspace_bytes(size_t n, uint64_t num_rows) {
-  return 4 * ((size_t)num_rows + 1 + 4 * n + sort_count_words(n, 1u << plan_for(num_rows).digit));
+size_t ugk_take_rows_grad_workspace_bytes(size_t n, uint64_t num_rows, size_t dim) {
+  return 4 * ((size_t)num_rows + 1 + 4 * n + 2 * pieces_of(n) * dim + sort_count_words(n, 1u << plan_for(num_rows).digit));
 }
 int ugk_take_rows_grad_i32(const void *grad_dev, size_t stride, const int32_t *index_dev, size_t n, uint64_t num_rows, size_t dim, int elem,
                            void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream) {

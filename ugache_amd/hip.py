@@ -160,7 +160,7 @@ SIGNATURES = {
     "ugk_expert_combine_grad": [_vp, _sz, _vp, _sz, _vp, _vp, _sz, _u32, _vp, C.c_int, _sz, C.c_int, _vp, _vp, _vp],
     "ugk_take_rows_i32": [_vp, _u64, _sz, _vp, _sz, _sz, C.c_int, _vp, _vp],
     "ugk_take_rows_i64": [_vp, _u64, _sz, _vp, _sz, _sz, C.c_int, _vp, _vp],
-    "ugk_take_rows_grad_workspace_bytes": [_sz, _u64],
+    "ugk_take_rows_grad_workspace_bytes": [_sz, _u64, _sz],
     "ugk_take_rows_grad_i32": [_vp, _sz, _vp, _sz, _u64, _sz, C.c_int, _vp, _vp, _sz, _vp],
     "ugk_take_rows_grad_i64": [_vp, _sz, _vp, _sz, _u64, _sz, C.c_int, _vp, _vp, _sz, _vp],
     "ugk_grad_norm_workspace_bytes": [_vp, _sz],
