@@ -34,8 +34,8 @@ def tensors(*entries):
     ("ugk_expert_sort_i32", (P, 1 << 31, 8, P, P, P, P, WS, None), "31 bits"),
     ("ugk_expert_sort_i32", (None, 8, 8, P, P, P, P, WS, None), "null pointer"),
     ("ugk_expert_sort_i32", (P, 8, 8, P, P, None, P, WS, None), "null pointer"),
-    ("ugk_expert_sort_i32", (P, 8, 8, P, P, P, P, 3, None), "workspace of 3 bytes"),
-    ("ugk_expert_sort_i32", (P, 8, 8, P, P, P, None, WS, None), "workspace"),
+    ("ugk_expert_sort_i32", (P, 100_000, 8, P, P, P, P, 3, None), "workspace of 3 bytes"),
+    ("ugk_expert_sort_i32", (P, 100_000, 8, P, P, P, None, WS, None), "workspace"),
     ("ugk_expert_dispatch", (P, 64, P, P, 4, 2, 64, 3, P, None), "element code 3"),
     ("ugk_expert_dispatch", (P, 64, P, P, 4, 0, 64, 4, P, None), "assignments"),
     ("ugk_expert_dispatch", (P, 64, P, P, 1 << 30, 2, 64, 4, P, None), "31 bits"),

@@ -104,9 +104,9 @@ def coll_torch_expert_sort(expert_ids, num_experts):
     src = torch.empty(n, dtype=torch.int32, device=where)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=where)
     nbytes = _L.ugk_expert_sort_workspace_bytes(n, num_experts)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=where)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=where) if nbytes else None
     _launch(_L.ugk_expert_sort_i64 if ids.dtype == torch.int64 else _L.ugk_expert_sort_i32, ids.get_device(), ids.data_ptr(), n,
-            num_experts, slot.data_ptr(), src.data_ptr(), offsets.data_ptr(), workspace.data_ptr(), nbytes)
+            num_experts, slot.data_ptr(), src.data_ptr(), offsets.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes)
     return ExpertOrder(slot, src, offsets)
 
 

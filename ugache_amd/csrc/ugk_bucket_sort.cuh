@@ -13,9 +13,7 @@ namespace ugk {
 namespace {
 
 constexpr int kSortBlock = 512, kSortWaves = kSortBlock / kWave;
-constexpr int kSortItems = 8;
-constexpr int kSortTile = kSortBlock * kSortItems;
-constexpr uint32_t kMaxBuckets = 1024;
+constexpr uint32_t kMaxBuckets = 2 * kSortBlock;  // a lane keeps the counts of two buckets
 constexpr uint32_t kNoBucket = 0xffffffffu;
 
 // kExperts: entries outside [0, buckets) have no bucket; kFirst: the lowest digit of an index, rows where it is outside [0,
@@ -51,14 +49,14 @@ __device__ __forceinline__ uint64_t same_bucket(uint32_t bucket, bool has, uint3
   return same;
 }
 
-// exclusive prefix sums of `count` words over a workgroup of kSortBlock lanes, in place; -> the total
-__device__ __forceinline__ uint32_t block_prefix(uint32_t *v, uint32_t count, uint32_t *wave_sum) {
-  const uint32_t per = (count + kSortBlock - 1) / kSortBlock;  // consecutive words of a lane
-  const uint32_t first = threadIdx.x * per;
-  uint32_t sum = 0;
-  for (uint32_t i = 0; i < per; ++i) sum += first + i < count ? v[first + i] : 0u;
-  uint32_t upto = sum;
+// Where the counts of the other tiles come from.  kSingle: there is one tile.  kFew: counts[tile][bucket], which every
+// workgroup adds up by itself.  kMany: a launch in between has added them up.
+enum Reach { kSingle, kFew, kMany };
+
+// the sum of a value over the lanes of the workgroup in front of this one, and over all of them
+__device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t &total, uint32_t *wave_sum) {
   const unsigned lane = lane_id();
+  uint32_t upto = v;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
     const uint32_t o = __shfl_up(upto, d);
@@ -66,55 +64,51 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t *v, uint32_t count, ui
   }
   if (lane == kWave - 1) wave_sum[threadIdx.x / kWave] = upto;
   __syncthreads();
-  uint32_t before = 0, total = 0;
+  uint32_t before = 0;
+  total = 0;
 #pragma unroll
   for (int w = 0; w < kSortWaves; ++w) {
     if (w < (int)(threadIdx.x / kWave)) before += wave_sum[w];
     total += wave_sum[w];
   }
-  uint32_t at = before + upto - sum;
-  for (uint32_t i = 0; i < per; ++i)
-    if (first + i < count) {
-      const uint32_t c = v[first + i];
-      v[first + i] = at;
-      at += c;
-    }
-  __syncthreads();
-  return total;
+  return before + upto - v;
 }
 
-// counts[bucket * tiles + tile]
-template <Pass P, typename K>
+// counts[tile * buckets + bucket], for kMany counts[bucket * tiles + tile]
+template <Pass P, typename K, int ITEMS, Reach R>
 __global__ __launch_bounds__(kSortBlock) void sort_count_kernel(const K *__restrict__ keys, size_t n, Digits d,
                                                                 uint32_t *__restrict__ counts) {
   __shared__ uint32_t count[kMaxBuckets];
+  const size_t base = (size_t)blockIdx.x * (kSortBlock * ITEMS) + threadIdx.x;
+  uint32_t key[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const size_t i = base + (size_t)j * kSortBlock;
+    key[j] = i < n ? sort_key<P>(keys, i, d) : kNoBucket;
+  }
   for (uint32_t b = threadIdx.x; b < d.buckets; b += kSortBlock) count[b] = 0;
   __syncthreads();
-  const size_t base = (size_t)blockIdx.x * kSortTile;
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const size_t i = base + (size_t)j * kSortBlock + threadIdx.x;
-    if (i < n) {
-      const uint32_t key = sort_key<P>(keys, i, d);
-      if (P != kExperts || key != kNoBucket) atomicAdd(&count[sort_bucket<P>(key, d)], 1u);
-    }
+  for (int j = 0; j < ITEMS; ++j) {
+    const size_t i = base + (size_t)j * kSortBlock;
+    if (i < n && (P != kExperts || key[j] != kNoBucket)) atomicAdd(&count[sort_bucket<P>(key[j], d)], 1u);
   }
   __syncthreads();
-  for (uint32_t b = threadIdx.x; b < d.buckets; b += kSortBlock) counts[(size_t)b * gridDim.x + blockIdx.x] = count[b];
+  for (uint32_t b = threadIdx.x; b < d.buckets; b += kSortBlock)
+    counts[R == kMany ? (size_t)b * gridDim.x + blockIdx.x : (size_t)blockIdx.x * d.buckets + b] = count[b];
 }
 
 // workgroup b: before[tile * buckets + b] = entries of bucket b in earlier tiles; totals[b]
 __global__ __launch_bounds__(kSortBlock) void sort_prefix_kernel(const uint32_t *__restrict__ counts, uint32_t tiles, uint32_t buckets,
                                                                  uint32_t *__restrict__ before, uint32_t *__restrict__ totals) {
-  __shared__ uint32_t part[kSortBlock], wave_sum[kSortWaves];
+  __shared__ uint32_t wave_sum[kSortWaves];
   const uint32_t b = blockIdx.x;
   uint32_t so_far = 0;
   for (uint32_t t0 = 0; t0 < tiles; t0 += kSortBlock) {
     const uint32_t t = t0 + threadIdx.x;
-    part[threadIdx.x] = t < tiles ? counts[(size_t)b * tiles + t] : 0u;
-    __syncthreads();
-    const uint32_t sum = block_prefix(part, kSortBlock, wave_sum);
-    if (t < tiles) before[(size_t)t * buckets + b] = so_far + part[threadIdx.x];
+    uint32_t sum;
+    const uint32_t at = block_before(t < tiles ? counts[(size_t)b * tiles + t] : 0u, sum, wave_sum);
+    if (t < tiles) before[(size_t)t * buckets + b] = so_far + at;
     so_far += sum;
     __syncthreads();
   }
@@ -123,32 +117,51 @@ __global__ __launch_bounds__(kSortBlock) void sort_prefix_kernel(const uint32_t 
 
 // kExperts: slot[i], src[position], offsets[buckets + 1]; src is -1 behind the last position.  kFirst, kNext: key_out and
 // entry_out at the position; entry is i in the first pass and entries[i] in the others.
-template <Pass P, typename K>
+template <Pass P, typename K, int ITEMS, Reach R>
 __global__ __launch_bounds__(kSortBlock) void sort_place_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ entries, size_t n,
-                                                                Digits d, const uint32_t *__restrict__ before,
+                                                                Digits d, const uint32_t *__restrict__ counts,
                                                                 const uint32_t *__restrict__ totals, uint32_t *__restrict__ out0,
                                                                 uint32_t *__restrict__ out1, uint32_t *__restrict__ offsets) {
-  __shared__ uint32_t base[kMaxBuckets];
   __shared__ uint32_t seen[kSortWaves][kMaxBuckets];
   __shared__ uint32_t wave_sum[kSortWaves];
-  for (uint32_t b = threadIdx.x; b < d.buckets; b += kSortBlock) {
-    base[b] = totals[b];
-#pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) seen[w][b] = 0;
-  }
-  __syncthreads();
-  const uint32_t total = block_prefix(base, d.buckets, wave_sum);
   const unsigned lane = lane_id(), wave = wave_in_block();
-  const uint64_t below = (1ull << lane) - 1ull;
-  const size_t tile0 = (size_t)blockIdx.x * kSortTile, first = tile0 + (size_t)wave * (kWave * kSortItems) + lane;
-  uint32_t key[kSortItems], rank[kSortItems];
+  const size_t first = (size_t)blockIdx.x * (kSortBlock * ITEMS) + (size_t)wave * (kWave * ITEMS) + lane;
+  // everything that is read is on its way before the first of it is waited for
+  uint32_t key[ITEMS], entry[ITEMS], rank[ITEMS];
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
+  for (int j = 0; j < ITEMS; ++j) {
     const size_t i = first + (size_t)j * kWave;
     key[j] = i < n ? sort_key<P>(keys, i, d) : kNoBucket;
+    entry[j] = P == kNext && i < n ? entries[i] : (uint32_t)i;
+  }
+  const uint32_t mine = 2 * threadIdx.x;  // this lane's two buckets
+  uint32_t before[2] = {0, 0}, all[2] = {0, 0};
+  if constexpr (R == kMany) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (mine + h < d.buckets) {
+        before[h] = counts[(size_t)blockIdx.x * d.buckets + mine + h];
+        all[h] = totals[mine + h];
+      }
+  } else if constexpr (R == kFew) {
+#pragma unroll 8
+    for (uint32_t t = 0; t < gridDim.x; ++t) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (mine + h < d.buckets) {
+          const uint32_t c = counts[t * d.buckets + mine + h];
+          all[h] += c;
+          before[h] += t < blockIdx.x ? c : 0u;
+        }
+    }
   }
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
+  for (int w = 0; w < kSortWaves; ++w)
+    for (uint32_t b = threadIdx.x; b < d.buckets; b += kSortBlock) seen[w][b] = 0;
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1ull;
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
     const size_t i = first + (size_t)j * kWave;
     const bool has = i < n && (P != kExperts || key[j] != kNoBucket);
     const uint32_t bucket = has ? sort_bucket<P>(key[j], d) : 0u;
@@ -163,20 +176,32 @@ __global__ __launch_bounds__(kSortBlock) void sort_place_kernel(const K *__restr
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  for (uint32_t b = threadIdx.x; b < d.buckets; b += kSortBlock) {
-    if (P == kExperts && blockIdx.x == 0) offsets[b] = base[b];
-    uint32_t at = base[b] + before[(size_t)blockIdx.x * d.buckets + b];
+  if constexpr (R == kSingle) {
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = seen[w][b];
-      seen[w][b] = at;
-      at += c;
-    }
+    for (int h = 0; h < 2; ++h)
+      if (mine + h < d.buckets)
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) all[h] += seen[w][mine + h];
   }
+  uint32_t total;
+  const uint32_t base = block_before(all[0] + all[1], total, wave_sum);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (mine + h < d.buckets) {
+      uint32_t at = base + (h ? all[0] : 0u);
+      if (P == kExperts && blockIdx.x == 0) offsets[mine + h] = at;
+      at += before[h];
+#pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) {
+        const uint32_t c = seen[w][mine + h];
+        seen[w][mine + h] = at;
+        at += c;
+      }
+    }
   if (P == kExperts && blockIdx.x == 0 && threadIdx.x == 0) offsets[d.buckets] = total;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
+  for (int j = 0; j < ITEMS; ++j) {
     const size_t i = first + (size_t)j * kWave;
     if (i >= n) continue;
     if constexpr (P == kExperts) {
@@ -188,7 +213,7 @@ __global__ __launch_bounds__(kSortBlock) void sort_place_kernel(const K *__restr
     } else {
       const uint32_t at = seen[wave][sort_bucket<P>(key[j], d)] + rank[j];
       out0[at] = key[j];
-      out1[at] = P == kFirst ? (uint32_t)i : entries[i];
+      out1[at] = entry[j];
     }
   }
 }
@@ -198,21 +223,49 @@ static inline uint32_t bits_for(uint64_t values) {  // that tell `values` number
   while (((uint64_t)1 << bits) < values) ++bits;
   return bits;
 }
-static inline size_t sort_tiles(size_t n) { return (n + kSortTile - 1) / kSortTile; }
+// How a pass goes by its size.
+struct SortShape {
+  int items;
+  Reach reach;
+  uint32_t tiles;
+};
+static inline SortShape sort_shape(size_t n) {
+  const auto tiles = [n](int items) { return (uint32_t)((n + kSortBlock * items - 1) / (kSortBlock * items)); };
+  if (n <= 2 * kSortBlock) return SortShape{2, kSingle, 1};
+  if (n <= 8 * kSortBlock) return SortShape{8, kSingle, 1};
+  if (tiles(2) <= 16) return SortShape{2, kFew, tiles(2)};
+  if (tiles(8) <= 32) return SortShape{8, kFew, tiles(8)};
+  return SortShape{8, kMany, tiles(8)};
+}
 // words of the counts of a pass: of every tile, summed over the tiles before, and of all
-static inline size_t sort_count_words(size_t n, uint32_t buckets) { return (2 * sort_tiles(n) + 1) * (size_t)buckets; }
+static inline size_t sort_count_words(size_t n, uint32_t buckets) {
+  const SortShape s = sort_shape(n);
+  return s.reach == kSingle ? 0 : s.reach == kFew ? (size_t)s.tiles * buckets : (2 * (size_t)s.tiles + 1) * buckets;
+}
+
+template <Pass P, typename K, int ITEMS, Reach R>
+static inline int sort_pass_as(const K *keys, const uint32_t *entries, size_t n, const Digits &d, uint32_t tiles, uint32_t *words,
+                               uint32_t *out0, uint32_t *out1, uint32_t *offsets, hipStream_t stream) {
+  uint32_t *counts = words, *before = counts + (size_t)tiles * d.buckets, *totals = before + (size_t)tiles * d.buckets;
+  if constexpr (R != kSingle)
+    hipLaunchKernelGGL((sort_count_kernel<P, K, ITEMS, R>), dim3(tiles), dim3(kSortBlock), 0, stream, keys, n, d, counts);
+  if constexpr (R == kMany)
+    hipLaunchKernelGGL(sort_prefix_kernel, dim3(d.buckets), dim3(kSortBlock), 0, stream, counts, tiles, d.buckets, before, totals);
+  hipLaunchKernelGGL((sort_place_kernel<P, K, ITEMS, R>), dim3(tiles), dim3(kSortBlock), 0, stream, keys, entries, n, d,
+                     R == kMany ? before : counts, totals, out0, out1, offsets);
+  UGK_HIP(hipGetLastError());
+  return 0;
+}
 
 template <Pass P, typename K>
 static inline int sort_pass(const K *keys, const uint32_t *entries, size_t n, const Digits &d, uint32_t *words, uint32_t *out0,
                             uint32_t *out1, uint32_t *offsets, hipStream_t stream) {
-  const size_t tiles = sort_tiles(n);
-  uint32_t *counts = words, *before = counts + tiles * d.buckets, *totals = before + tiles * d.buckets;
-  hipLaunchKernelGGL((sort_count_kernel<P, K>), dim3((unsigned)tiles), dim3(kSortBlock), 0, stream, keys, n, d, counts);
-  hipLaunchKernelGGL(sort_prefix_kernel, dim3(d.buckets), dim3(kSortBlock), 0, stream, counts, (uint32_t)tiles, d.buckets, before, totals);
-  hipLaunchKernelGGL((sort_place_kernel<P, K>), dim3((unsigned)tiles), dim3(kSortBlock), 0, stream, keys, entries, n, d, before, totals, out0,
-                     out1, offsets);
-  UGK_HIP(hipGetLastError());
-  return 0;
+  const SortShape s = sort_shape(n);
+  if (s.reach == kMany) return sort_pass_as<P, K, 8, kMany>(keys, entries, n, d, s.tiles, words, out0, out1, offsets, stream);
+  if (s.reach == kFew && s.items == 8) return sort_pass_as<P, K, 8, kFew>(keys, entries, n, d, s.tiles, words, out0, out1, offsets, stream);
+  if (s.reach == kFew) return sort_pass_as<P, K, 2, kFew>(keys, entries, n, d, s.tiles, words, out0, out1, offsets, stream);
+  if (s.items == 8) return sort_pass_as<P, K, 8, kSingle>(keys, entries, n, d, 1, words, out0, out1, offsets, stream);
+  return sort_pass_as<P, K, 2, kSingle>(keys, entries, n, d, 1, words, out0, out1, offsets, stream);
 }
 
 }  // namespace

@@ -116,8 +116,9 @@ int expert_sort(const K *ids, size_t n, uint32_t num_experts, int32_t *slot, int
   UGK_REQUIRE(n < ((size_t)1 << 31), "ugk_expert_sort: %zu assignments, positions have 31 bits", n);
   UGK_REQUIRE(offsets && (n == 0 || (ids && slot && src)), "ugk_expert_sort: null pointer");
   if (n == 0) return ugk_fill_u32(reinterpret_cast<uint32_t *>(offsets), 0, (size_t)num_experts + 1, stream);
-  UGK_REQUIRE(workspace && workspace_bytes >= ugk_expert_sort_workspace_bytes(n, num_experts),
-              "ugk_expert_sort: a workspace of %zu bytes, %zu are needed", workspace_bytes, ugk_expert_sort_workspace_bytes(n, num_experts));
+  const size_t need = ugk_expert_sort_workspace_bytes(n, num_experts);
+  UGK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "ugk_expert_sort: a workspace of %zu bytes, %zu are needed", workspace_bytes,
+              need);
   const Digits d{0, 0, 0, num_experts, bits_for(num_experts)};
   return sort_pass<kExperts, K>(ids, nullptr, n, d, static_cast<uint32_t *>(workspace), reinterpret_cast<uint32_t *>(slot),
                                 reinterpret_cast<uint32_t *>(src), reinterpret_cast<uint32_t *>(offsets), as_stream(stream));
