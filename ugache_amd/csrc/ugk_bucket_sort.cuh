@@ -136,24 +136,37 @@ __global__ __launch_bounds__(kSortBlock) void sort_place_kernel(const K *__restr
   }
   const uint32_t mine = 2 * threadIdx.x;  // this lane's two buckets
   uint32_t before[2] = {0, 0}, all[2] = {0, 0};
+  const uint32_t at0 = min(mine, d.buckets - 1), at1 = min(mine + 1, d.buckets - 1);
   if constexpr (R == kMany) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (mine + h < d.buckets) {
-        before[h] = counts[(size_t)blockIdx.x * d.buckets + mine + h];
-        all[h] = totals[mine + h];
-      }
+    before[0] = counts[(size_t)blockIdx.x * d.buckets + at0];
+    before[1] = counts[(size_t)blockIdx.x * d.buckets + at1];
+    all[0] = totals[at0];
+    all[1] = totals[at1];
   } else if constexpr (R == kFew) {
-#pragma unroll 8
-    for (uint32_t t = 0; t < gridDim.x; ++t) {
+    // sixteen tiles at a time and no branch in between: their counts come out of other XCDs' caches, a microsecond and a
+    // half each if they are waited for one by one (16,384 entries in 16 tiles: 11.1 -> 5 us)
+    constexpr uint32_t U = 16;
+    for (uint32_t t0 = 0; t0 < gridDim.x; t0 += U) {
+      uint32_t c[U][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (mine + h < d.buckets) {
-          const uint32_t c = counts[t * d.buckets + mine + h];
-          all[h] += c;
-          before[h] += t < blockIdx.x ? c : 0u;
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t *of = counts + min(t0 + u, gridDim.x - 1) * d.buckets;
+        c[u][0] = of[at0];
+        c[u][1] = of[at1];
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          all[h] += t0 + u < gridDim.x ? c[u][h] : 0u;
+          before[h] += t0 + u < blockIdx.x ? c[u][h] : 0u;
         }
     }
+  }
+  if constexpr (R != kSingle) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (mine + h >= d.buckets) all[h] = 0;
   }
 #pragma unroll
   for (int w = 0; w < kSortWaves; ++w)

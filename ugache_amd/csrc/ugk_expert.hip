@@ -44,15 +44,29 @@ __global__ __launch_bounds__(kBlock) void combine_kernel(const T *__restrict__ r
   if (t >= tokens) return;
   const uint32_t at = min(c * VEC, dim - VEC);
   float sum[VEC] = {};
-  for (uint32_t k = 0; k < top; ++k) {
-    const size_t i = t * top + k;
-    const uint32_t s = (uint32_t)slot[i];
-    if (s >= n_rows) continue;
-    const float w = weights ? load_weight(weights, weight_elem, i) : 1.f;
-    float v[VEC];
-    load_chunk<T, VEC>(rows + s * stride + at, v);
+  constexpr uint32_t U = 8;  // rows on their way
+  for (uint32_t k0 = 0; k0 < top; k0 += U) {
+    const size_t i = t * top + k0;
+    const uint32_t last = min(U, top - k0) - 1;
+    uint32_t s[U];
+    float w[U];
+    typename ChunkOf<T, VEC>::type v[U];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) sum[e] = fmaf(w, v[e], sum[e]);
+    for (uint32_t u = 0; u < U; ++u) {
+      s[u] = (uint32_t)slot[i + min(u, last)];
+      w[u] = weights ? load_weight(weights, weight_elem, i + min(u, last)) : 1.f;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+      if (u <= last && s[u] < n_rows) v[u] = raw_chunk<T, VEC>(rows + s[u] * stride + at);
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+      if (u <= last && s[u] < n_rows) {
+        float x[VEC];
+        to_floats<T, VEC>(v[u], x);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] = fmaf(w[u], x[e], sum[e]);
+      }
   }
   store_chunk<T, VEC>(out + t * dim + at, sum);
 }
@@ -129,7 +143,7 @@ int check_rows(const char *what, size_t tokens, uint32_t top, size_t dim, int el
   UGK_REQUIRE(elem_ok(elem), "%s: element code %d is none of fp32 (4), fp16 (2) and bfloat16 (UGK_ELEM_BF16)", what, elem);
   UGK_REQUIRE(top >= 1 && tokens < ((size_t)1 << 31) && tokens * top < ((size_t)1 << 31),
               "%s: %zu tokens of %u assignments, positions have 31 bits", what, tokens, top);
-  UGK_REQUIRE(dim >= 1 && dim < ((size_t)1 << 30), "%s: rows of %zu elements", what, dim);
+  UGK_REQUIRE(dim >= 1 && dim < kMaxDim, "%s: rows of %zu elements", what, dim);
   UGK_REQUIRE(stride >= dim || tokens <= 1, "%s: rows of %zu elements overlap at a stride of %zu", what, dim, stride);
   return 0;
 }

@@ -10,53 +10,84 @@ namespace {
 
 // What a launch is told of its tensors travels in its arguments (the list of a training step changes with every step):
 // up to kListed tensors at a time, each a run of consecutive pieces.
-constexpr int kListed = 120;
+constexpr int kListed = 110;
 constexpr uint32_t kPieceBytes = 32768;
+struct Listed {
+  const void *data;
+  void *out;
+  uint64_t count;
+  int32_t elem;
+};
 struct TensorList {
-  const void *data[kListed];
-  void *out[kListed];
-  uint64_t count[kListed];
-  uint32_t first[kListed];  // the tensor's first piece in this launch
-  int32_t elem[kListed];
-  uint32_t n;
+  Listed tensor[kListed];
+  uint32_t first[kListed];  // a tensor's first piece in this launch
+  uint32_t n, pieces;
 };
 
-static inline uint64_t pieces_of(const ugk_tensor_t &t) { return (t.count * elem_size(t.elem) + kPieceBytes - 1) / kPieceBytes; }
+__host__ __device__ static inline uint32_t pieces_of(uint64_t count, int elem) {
+  return (uint32_t)((count * (elem == 4 ? 4 : 2) + kPieceBytes - 1) / kPieceBytes);
+}
+static inline uint64_t pieces_of(const ugk_tensor_t &t) { return pieces_of(t.count, t.elem); }
 
+// the tensor of a piece: how many of the first pieces are not behind it
 __device__ __forceinline__ uint32_t tensor_of(const TensorList &list, uint32_t piece) {
-  uint32_t at = 0;
-  for (uint32_t i = 1; i < list.n; ++i) at += list.first[i] <= piece ? 1u : 0u;
-  return at;
+  uint32_t found = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kListed; i += kWave) {
+    const uint32_t at = i + lane_id();
+    found += (uint32_t)__popcll(__ballot(at < list.n && list.first[min(at, (uint32_t)kListed - 1)] <= piece));
+  }
+  return __builtin_amdgcn_readfirstlane(found - 1);
 }
 
+// f for the 16-byte chunks of a piece, all of a lane's on their way at once where the piece is a whole one, and for the
+// elements behind the last chunk
 template <typename T, typename F>
 __device__ __forceinline__ void for_elements(const T *data, uint64_t count, uint32_t piece, F f) {
-  constexpr int VEC = 16 / sizeof(T);
+  constexpr int VEC = 16 / sizeof(T), U = kPieceBytes / (16 * kBlock);
   constexpr uint32_t kElems = kPieceBytes / sizeof(T);
   const uint64_t begin = (uint64_t)piece * kElems;
-  const uint32_t n = (uint32_t)min((uint64_t)kElems, count - begin);
+  // (a shift and not min(): of a 64-bit minimum in scalar registers that a branch depends on as well, this compiler makes a
+  // select without its condition)
+  const uint64_t left = count - begin;
+  const bool whole = left / kElems != 0;
+  const uint32_t n = whole ? kElems : (uint32_t)left;
+  const T *from = data + begin;
+  if (whole) {
+    typename ChunkOf<T, VEC>::type v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = raw_chunk<T, VEC>(from + (u * kBlock + threadIdx.x) * VEC);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[VEC];
+      to_floats<T, VEC>(v[u], x);
+      f(begin + (u * kBlock + threadIdx.x) * VEC, x, std::integral_constant<int, VEC>());
+    }
+    return;
+  }
   for (uint32_t i = threadIdx.x * VEC; i + VEC <= n; i += kBlock * VEC) {
     float x[VEC];
-    load_chunk<T, VEC>(data + begin + i, x);
+    load_chunk<T, VEC>(from + i, x);
     f(begin + i, x, std::integral_constant<int, VEC>());
   }
   const uint32_t tail = n / VEC * VEC + threadIdx.x;
   if (tail < n) {
     float x[1];
-    load_chunk<T, 1>(data + begin + tail, x);
+    load_chunk<T, 1>(from + tail, x);
     f(begin + tail, x, std::integral_constant<int, 1>());
   }
 }
 
+template <int BLOCK>
 __device__ __forceinline__ double block_sum(double v) {
-  __shared__ double wave_sum[kBlock / kWave];
+  __shared__ double wave_sum[BLOCK / kWave];
 #pragma unroll
   for (int d = kWave / 2; d > 0; d /= 2) v += __shfl_xor(v, d);
   if (lane_id() == 0) wave_sum[wave_in_block()] = v;
   __syncthreads();
   double sum = 0;
 #pragma unroll
-  for (int w = 0; w < kBlock / kWave; ++w) sum += wave_sum[w];
+  for (int w = 0; w < BLOCK / kWave; ++w) sum += wave_sum[w];
   return sum;
 }
 
@@ -71,20 +102,29 @@ __device__ __forceinline__ double squares(const void *data, uint64_t count, uint
 }
 
 __global__ __launch_bounds__(kBlock) void grad_squares_kernel(TensorList list, double *__restrict__ sums) {
-  const uint32_t t = tensor_of(list, blockIdx.x), piece = blockIdx.x - list.first[t];
-  const double mine = list.elem[t] == 4   ? squares<float>(list.data[t], list.count[t], piece)
-                      : list.elem[t] == 2 ? squares<half_t>(list.data[t], list.count[t], piece)
-                                          : squares<bhalf_t>(list.data[t], list.count[t], piece);
-  const double sum = block_sum(mine);
+  const uint32_t at = tensor_of(list, blockIdx.x), piece = blockIdx.x - list.first[at];
+  const Listed t = list.tensor[at];
+  const double mine = t.elem == 4   ? squares<float>(t.data, t.count, piece)
+                      : t.elem == 2 ? squares<half_t>(t.data, t.count, piece)
+                                    : squares<bhalf_t>(t.data, t.count, piece);
+  const double sum = block_sum<kBlock>(mine);
   if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
 
 // one workgroup: the pieces' sums added up; total[0] = their sum
-__global__ __launch_bounds__(kBlock) void grad_norm_kernel(const double *__restrict__ sums, size_t pieces, double *__restrict__ total,
-                                                           float *__restrict__ norm) {
+constexpr int kNormBlock = 1024;
+__global__ __launch_bounds__(kNormBlock) void grad_norm_kernel(const double *__restrict__ sums, uint64_t pieces, double *__restrict__ total,
+                                                               float *__restrict__ norm) {
+  constexpr int U = 8;  // sums on their way
   double mine = 0;
-  for (size_t i = threadIdx.x; i < pieces; i += kBlock) mine += sums[i];
-  const double sum = block_sum(mine);
+  for (uint64_t i = threadIdx.x; i < pieces; i += U * kNormBlock) {
+    double v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = sums[min(i + u * kNormBlock, pieces - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) mine += i + u * kNormBlock < pieces ? v[u] : 0.0;
+  }
+  const double sum = block_sum<kNormBlock>(mine);
   if (threadIdx.x == 0) {
     *total = sum;
     *norm = (float)sqrt(sum);
@@ -109,11 +149,15 @@ __global__ __launch_bounds__(kBlock) void grad_scale_kernel(TensorList list, con
   // a factor near the end of float's range, which a norm beyond it brings, would lose its digits: it is multiplied in two steps
   const bool small = ratio < 0x1p-100;
   const float factor = ratio >= 1.0 ? 1.f : (float)(small ? ratio * 0x1p100 : ratio), after = small ? 0x1p-100f : 1.f;
-  const uint32_t t = tensor_of(list, blockIdx.x), piece = blockIdx.x - list.first[t];
-  if (factor == 1.f && list.out[t] == list.data[t]) return;
-  if (list.elem[t] == 4) scaled<float>(list.data[t], list.out[t], list.count[t], piece, factor, after);
-  else if (list.elem[t] == 2) scaled<half_t>(list.data[t], list.out[t], list.count[t], piece, factor, after);
-  else scaled<bhalf_t>(list.data[t], list.out[t], list.count[t], piece, factor, after);
+  // from the last piece to the first: the last ones read for the norm are the ones the memory-side cache still holds
+  // (the tensors are listed from the last to the first)
+  const uint32_t at = tensor_of(list, blockIdx.x);
+  const Listed t = list.tensor[at];
+  const uint32_t piece = pieces_of(t.count, t.elem) - 1 - (blockIdx.x - list.first[at]);
+  if (factor == 1.f && t.out == t.data) return;
+  if (t.elem == 4) scaled<float>(t.data, t.out, t.count, piece, factor, after);
+  else if (t.elem == 2) scaled<half_t>(t.data, t.out, t.count, piece, factor, after);
+  else scaled<bhalf_t>(t.data, t.out, t.count, piece, factor, after);
 }
 
 __global__ void preload_grad_norm_kernel() {}
@@ -123,29 +167,31 @@ void preload_grad_norm(hipStream_t stream) { hipLaunchKernelGGL(preload_grad_nor
 
 namespace {
 
-// calls launch(list, pieces of it, pieces before it) for the tensors in lists that fit a launch's arguments
+// calls launch(list, pieces before it) for the tensors in lists that fit a launch's arguments, from the last list to the
+// first where `backwards`
 template <typename F>
-int for_lists(const ugk_tensor_t *tensors, size_t n, F launch) {
+int for_lists(const ugk_tensor_t *tensors, size_t n, bool backwards, F launch) {
   TensorList list;
-  uint64_t pieces = 0, before = 0;
-  list.n = 0;
-  for (size_t i = 0; i <= n; ++i) {
-    const uint64_t more = i < n ? pieces_of(tensors[i]) : 0;
-    if (i < n && more == 0) continue;
-    if (list.n > 0 && (i == n || list.n == (uint32_t)kListed || pieces + more >= ((uint64_t)1 << 31))) {
-      if (int rc = launch(list, pieces, before)) return rc;
-      before += pieces, pieces = 0, list.n = 0;
-    }
-    if (i == n) break;
+  uint64_t before = 0;
+  list.n = list.pieces = 0;
+  const auto add = [&list](const ugk_tensor_t &t, uint64_t more) {
     const uint32_t at = list.n++;
-    list.data[at] = tensors[i].data;
-    list.out[at] = tensors[i].out ? tensors[i].out : const_cast<void *>(tensors[i].data);
-    list.count[at] = tensors[i].count;
-    list.first[at] = (uint32_t)pieces;
-    list.elem[at] = tensors[i].elem;
-    pieces += more;
+    list.tensor[at] = Listed{t.data, t.out ? t.out : const_cast<void *>(t.data), t.count, t.elem};
+    list.first[at] = list.pieces;
+    list.pieces += (uint32_t)more;
+  };
+  for (size_t k = 0; k < n; ++k) {
+    const ugk_tensor_t &t = tensors[backwards ? n - 1 - k : k];
+    const uint64_t more = pieces_of(t);
+    if (more == 0) continue;
+    if (list.n > 0 && (list.n == (uint32_t)kListed || list.pieces + more >= ((uint64_t)1 << 31))) {
+      if (int rc = launch(list, before)) return rc;
+      before += list.pieces;
+      list.n = list.pieces = 0;
+    }
+    add(t, more);
   }
-  return 0;
+  return list.n > 0 ? launch(list, before) : 0;
 }
 
 int grad_norm(const char *what, const ugk_tensor_t *tensors, size_t n, void *workspace, size_t workspace_bytes, float *norm, hipStream_t stream) {
@@ -155,20 +201,20 @@ int grad_norm(const char *what, const ugk_tensor_t *tensors, size_t n, void *wor
     UGK_REQUIRE(elem_ok(tensors[i].elem), "%s: element code %d of tensor %zu is none of fp32 (4), fp16 (2) and bfloat16 (UGK_ELEM_BF16)", what,
                 tensors[i].elem, i);
     UGK_REQUIRE(tensors[i].data || tensors[i].count == 0, "%s: null data of tensor %zu", what, i);
-    UGK_REQUIRE(tensors[i].count < ((uint64_t)1 << 44), "%s: %zu elements in tensor %zu", what, (size_t)tensors[i].count, i);
+    UGK_REQUIRE(tensors[i].count < ((uint64_t)1 << 42), "%s: %zu elements in tensor %zu", what, (size_t)tensors[i].count, i);
     pieces += pieces_of(tensors[i]);
   }
   UGK_REQUIRE(norm, "%s: null output", what);
   UGK_REQUIRE(workspace && workspace_bytes >= (pieces + 1) * sizeof(double), "%s: a workspace of %zu bytes, %zu are needed", what, workspace_bytes,
               (size_t)(pieces + 1) * sizeof(double));
   double *total = static_cast<double *>(workspace), *sums = total + 1;
-  const int rc = for_lists(tensors, n, [&](const TensorList &list, uint64_t count, uint64_t before) -> int {
-    hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)count), dim3(kBlock), 0, stream, list, sums + before);
+  const int rc = for_lists(tensors, n, false, [&](const TensorList &list, uint64_t before) -> int {
+    hipLaunchKernelGGL(grad_squares_kernel, dim3(list.pieces), dim3(kBlock), 0, stream, list, sums + before);
     UGK_HIP(hipGetLastError());
     return 0;
   });
   if (rc) return rc;
-  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, stream, sums, (size_t)pieces, total, norm);
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kNormBlock), 0, stream, sums, pieces, total, norm);
   UGK_HIP(hipGetLastError());
   return 0;
 }
@@ -194,8 +240,8 @@ int ugk_grad_clip(const ugk_tensor_t *tensors, size_t n, double max_norm, void *
                   void *stream) {
   UGK_REQUIRE(max_norm >= 0, "ugk_grad_clip: a limit of %g", max_norm);
   if (int rc = grad_norm("ugk_grad_clip", tensors, n, workspace_dev, workspace_bytes, norm_dev, as_stream(stream))) return rc;
-  return for_lists(tensors, n, [&](const TensorList &list, uint64_t count, uint64_t) -> int {
-    hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)count), dim3(kBlock), 0, as_stream(stream), list,
+  return for_lists(tensors, n, true, [&](const TensorList &list, uint64_t) -> int {
+    hipLaunchKernelGGL(grad_scale_kernel, dim3(list.pieces), dim3(kBlock), 0, as_stream(stream), list,
                        static_cast<const double *>(workspace_dev), max_norm);
     UGK_HIP(hipGetLastError());
     return 0;

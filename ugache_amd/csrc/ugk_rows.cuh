@@ -28,14 +28,22 @@ struct ChunkOf<T, 1> {
 };
 
 template <typename T, int VEC>
-__device__ __forceinline__ void load_chunk(const T *from, float (&x)[VEC]) {
-  const typename ChunkOf<T, VEC>::type v = *reinterpret_cast<const typename ChunkOf<T, VEC>::type *>(from);
+__device__ __forceinline__ typename ChunkOf<T, VEC>::type raw_chunk(const T *from) {
+  return *reinterpret_cast<const typename ChunkOf<T, VEC>::type *>(from);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void to_floats(const typename ChunkOf<T, VEC>::type &v, float (&x)[VEC]) {
   if constexpr (VEC == 1) {
     x[0] = (float)v;
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) x[i] = (float)v[i];
   }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_chunk(const T *from, float (&x)[VEC]) {
+  to_floats<T, VEC>(raw_chunk<T, VEC>(from), x);
 }
 
 template <typename T, int VEC>
@@ -73,15 +81,15 @@ static inline Split split_of(size_t dim, int vec) {
 }
 static inline size_t split_blocks(size_t rows, const Split &s) { return (rows * s.chunks + kBlock - 1) / kBlock; }
 
-// the row and the chunk of a lane.  The division of the workgroup's first number is scalar; what a lane adds to its remainder
-// stays below chunks + 256, where the product with the magic number is exact for up to 256 chunks and a comparison does
-// for more.
+// The row and the chunk of a lane.  Every `chunks` workgroups take kBlock rows, so that 32 bits hold what is divided, and the
+// divisions are scalar; what a lane adds to the second remainder stays below chunks + kBlock, where the product with the
+// magic number is exact for up to kBlock chunks and a comparison does for more.
+constexpr size_t kMaxDim = (size_t)1 << 25;
 __device__ __forceinline__ void split_lane(const Split &s, uint32_t block, size_t &row, uint32_t &chunk) {
-  const uint64_t first = (uint64_t)block * kBlock;
-  const uint64_t row0 = first / s.chunks;
-  const uint32_t at = (uint32_t)(first - row0 * s.chunks) + threadIdx.x;
+  const uint32_t group = block / s.chunks, first = (block - group * s.chunks) * kBlock, row0 = first / s.chunks;
+  const uint32_t at = first - row0 * s.chunks + threadIdx.x;
   const uint32_t over = s.chunks == 1 ? at : s.chunks > (uint32_t)kBlock ? (at >= s.chunks ? 1u : 0u) : __umulhi(at, s.magic);
-  row = row0 + over;
+  row = (size_t)group * kBlock + (row0 + over);
   chunk = at - over * s.chunks;
 }
 

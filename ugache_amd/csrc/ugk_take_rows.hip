@@ -92,9 +92,9 @@ __global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ g
     return;
   }
   const uint32_t live = begin[rows];
-  const uint64_t first = i * kPiece;
-  if (first >= live) return;
-  const uint32_t from = (uint32_t)first, to = (uint32_t)min(first + kPiece, (uint64_t)live);
+  const uint32_t from = (uint32_t)i * kPiece;  // below n + kPiece
+  if (i * kPiece >= live) return;
+  const uint32_t to = min(from + kPiece, live);
   const uint32_t r0 = keys[from], begin0 = begin[r0], end0 = begin[r0 + 1];
   if (begin0 < from && end0 - begin0 > kPiece) {
     add_entries<T, VEC>(grad, stride, entries, from, min(to, end0), at, sum);
@@ -117,9 +117,9 @@ __global__ __launch_bounds__(kBlock) void row_join_kernel(const uint32_t *__rest
                                                           T *__restrict__ out) {
   __shared__ float held[kBlock * VEC];
   const uint32_t live = begin[rows];
-  const uint64_t first = (uint64_t)blockIdx.x * kPiece;
+  const uint32_t first = blockIdx.x * kPiece;  // below n
   if (first >= live) return;
-  const uint32_t r = keys[min(first + kPiece, (uint64_t)live) - 1], from = begin[r], to = begin[r + 1];
+  const uint32_t r = keys[min(first + kPiece, live) - 1], from = begin[r], to = begin[r + 1];
   if (from < first || to - from <= kPiece) return;
   const uint32_t group = threadIdx.x / lanes, groups = kBlock / lanes;  // lanes: a power of two
   const uint32_t c = blockIdx.y * lanes + threadIdx.x % lanes;
@@ -128,11 +128,19 @@ __global__ __launch_bounds__(kBlock) void row_join_kernel(const uint32_t *__rest
   const uint32_t per = (pieces + groups - 1) / groups;
   float sum[VEC] = {};
   if (c < chunks) {
-    for (uint32_t p = group * per; p < min((group + 1) * per, pieces); ++p) {
-      float v[VEC];
-      load_chunk<float, VEC>(parts + (2 * (size_t)(p0 + p) + (p == 0 ? 1 : 0)) * dim + at, v);
+    constexpr uint32_t U = 8;  // parts on their way
+    const uint32_t end = min((group + 1) * per, pieces);
+    for (uint32_t p = group * per; p < end; p += U) {
+      float v[U][VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e] += v[e];
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t q = min(p + u, end - 1);
+        load_chunk<float, VEC>(parts + (2 * (size_t)(p0 + q) + (q == 0 ? 1 : 0)) * dim + at, v[u]);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] += p + u < end ? v[u][e] : 0.f;
     }
   }
 #pragma unroll
@@ -155,7 +163,7 @@ namespace {
 template <typename I>
 int take_rows(const void *table, uint64_t num_rows, size_t stride, const I *index, size_t n, size_t dim, int elem, void *out, void *stream) {
   UGK_REQUIRE(elem_ok(elem), "ugk_take_rows: element code %d is none of fp32 (4), fp16 (2) and bfloat16 (UGK_ELEM_BF16)", elem);
-  UGK_REQUIRE(dim >= 1 && dim < ((size_t)1 << 30), "ugk_take_rows: rows of %zu elements", dim);
+  UGK_REQUIRE(dim >= 1 && dim < kMaxDim, "ugk_take_rows: rows of %zu elements", dim);
   UGK_REQUIRE(n < ((size_t)1 << 40) && num_rows < ((uint64_t)1 << 40), "ugk_take_rows: %zu of %zu rows", n, (size_t)num_rows);
   if (n == 0) return 0;
   UGK_REQUIRE((table || num_rows == 0) && index && out, "ugk_take_rows: null pointer");
@@ -188,7 +196,7 @@ template <typename I>
 int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, uint64_t num_rows, size_t dim, int elem, void *out,
                    void *workspace, size_t workspace_bytes, void *stream) {
   UGK_REQUIRE(elem_ok(elem), "ugk_take_rows_grad: element code %d is none of fp32 (4), fp16 (2) and bfloat16 (UGK_ELEM_BF16)", elem);
-  UGK_REQUIRE(dim >= 1 && dim < ((size_t)1 << 30), "ugk_take_rows_grad: rows of %zu elements", dim);
+  UGK_REQUIRE(dim >= 1 && dim < kMaxDim, "ugk_take_rows_grad: rows of %zu elements", dim);
   UGK_REQUIRE(n < ((size_t)1 << 31) && num_rows < ((uint64_t)1 << 31), "ugk_take_rows_grad: %zu entries of %zu rows, both have 31 bits", n,
               (size_t)num_rows);
   UGK_REQUIRE(stride >= dim || n <= 1, "ugk_take_rows_grad: rows of %zu elements overlap at a stride of %zu", dim, stride);
