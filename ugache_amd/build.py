@@ -6,6 +6,8 @@
 
   collcache/torch/c_lib_native.*.so — the compiled form of collcache.torch.c_lib (pybind11, g++), linked against
                       libcoll_cache.so.
+  collcache/torch/rows_native.*.so  — the calls of collcache.torch.rows (pybind11 and ATen, g++), linked against
+                      libugache_hip.so.
 
 All are built in-tree.  `python -m ugache_amd.build` rebuilds everything.
 """
@@ -115,10 +117,39 @@ def build_native_c_lib(verbose=False):
     return native_c_lib_path()
 
 
+def native_rows_path():
+    import sysconfig
+    return os.path.join(PKG, "collcache", "torch", "rows_native" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_native_rows(verbose=False):
+    """the extension module collcache.torch.rows_native over libugache_hip.so and torch's own libraries, which the process
+    that imports it has loaded already"""
+    import sysconfig
+
+    import torch
+    where = os.path.dirname(os.path.abspath(torch.__file__))
+    src = os.path.join(PKG, "collcache", "torch", "rows_native.cc")
+    out = _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+                "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+                "-I", INCLUDE, "-isystem", os.path.join(where, "include"),
+                "-isystem", os.path.join(where, "include", "torch", "csrc", "api", "include"),
+                "-I", sysconfig.get_paths()["include"], src, "-o", native_rows_path(), "-L", PKG, "-lugache_hip",
+                "-L", os.path.join(where, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN/../.."])
+    if verbose and out.strip():
+        print(out)
+    return native_rows_path()
+
+
 def build_all(verbose=False):
+    # the module over torch's headers takes as long as the longest kernel source: side by side with the rest
+    from concurrent.futures import ThreadPoolExecutor
     build_hip(verbose)
-    build_host(verbose)
-    build_native_c_lib(verbose)
+    with ThreadPoolExecutor(max_workers=1) as pool:
+        rows = pool.submit(build_native_rows, verbose)
+        build_host(verbose)
+        build_native_c_lib(verbose)
+        rows.result()
 
 
 if __name__ == "__main__":

@@ -11,7 +11,7 @@ namespace {
 // rows[slot[t, k]] = x[t] for every assignment of token t; the positions behind the last live one are zero rows, so that
 // what multiplies the whole buffer meets no stale bits.  The lane that holds a chunk of x[t] stores it `top` times; x is
 // read once.
-template <typename T, int VEC>
+template <typename T, int VEC, bool STREAM>
 __global__ __launch_bounds__(kBlock) void dispatch_kernel(const T *__restrict__ x, size_t x_stride, const int32_t *__restrict__ slot,
                                                           const int32_t *__restrict__ live, size_t tokens, uint32_t top,
                                                           uint32_t dim, Split split, T *__restrict__ rows) {
@@ -21,19 +21,19 @@ __global__ __launch_bounds__(kBlock) void dispatch_kernel(const T *__restrict__ 
   split_lane(split, blockIdx.x, t, c);
   if (t >= tokens) return;
   const uint32_t at = min(c * VEC, dim - VEC);
-  const chunk_t v = *reinterpret_cast<const chunk_t *>(x + t * x_stride + at);
-  const chunk_t zero = {};
+  const chunk_t v = raw_chunk<T, VEC>(x + t * x_stride + at), zero = {};
   const uint32_t n = (uint32_t)(tokens * top), n_live = (uint32_t)*live;
   for (uint32_t k = 0; k < top; ++k) {
     const uint32_t i = (uint32_t)t * top + k;
     const uint32_t s = (uint32_t)slot[i];
-    if (s < n) *reinterpret_cast<chunk_t *>(rows + (size_t)s * dim + at) = v;
-    if (i >= n_live) *reinterpret_cast<chunk_t *>(rows + (size_t)i * dim + at) = zero;
+    if (s < n) put_chunk<T, VEC, STREAM>(rows + (size_t)s * dim + at, v);
+    if (i >= n_live) put_chunk<T, VEC, STREAM>(rows + (size_t)i * dim + at, zero);
   }
 }
 
-// out[t] = sum over k of w[t, k] * rows[slot[t, k]], added in fp32 in the order of k by fused multiply-adds and rounded once
-template <typename T, int VEC>
+// out[t] = sum over k of w[t, k] * rows[slot[t, k]], added in fp32 in the order of k by fused multiply-adds and rounded once.
+// STREAM: the rows are more than the memory-side cache holds and are read past the caches.
+template <typename T, int VEC, bool STREAM>
 __global__ __launch_bounds__(kBlock) void combine_kernel(const T *__restrict__ rows, size_t stride, uint32_t n_rows,
                                                          const int32_t *__restrict__ slot, size_t tokens, uint32_t top,
                                                          const void *__restrict__ weights, int weight_elem, uint32_t dim,
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kBlock) void combine_kernel(const T *__restrict__ r
     }
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)
-      if (u <= last && s[u] < n_rows) v[u] = raw_chunk<T, VEC>(rows + s[u] * stride + at);
+      if (u <= last && s[u] < n_rows) v[u] = raw_chunk<T, VEC, STREAM>(rows + s[u] * stride + at);
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)
       if (u <= last && s[u] < n_rows) {
@@ -71,47 +71,91 @@ __global__ __launch_bounds__(kBlock) void combine_kernel(const T *__restrict__ r
   store_chunk<T, VEC>(out + t * dim + at, sum);
 }
 
-// a wavefront per token: grad_rows[slot] = w * grad_out[t], grad_weights[t, k] = <rows[slot], grad_out[t]>, positions
-// behind the last live one zero
-template <typename T, int VEC>
+// grad_rows[slot] = w * grad_out[t], grad_weights[t, k] = <rows[slot], grad_out[t]>, positions behind the last live one zero.
+// A group of `lanes` lanes, up to a wavefront, per token, or the whole workgroup (WIDE): it has U of the token's rows on
+// their way, CH chunks of each to a lane, and the chunks of grad_out that go with them.
+template <typename T, int VEC, bool STREAM, bool WIDE>
 __global__ __launch_bounds__(kBlock) void combine_grad_kernel(const T *__restrict__ grad_out, size_t grad_stride,
                                                               const T *__restrict__ rows, size_t stride,
                                                               const int32_t *__restrict__ slot, const int32_t *__restrict__ live,
                                                               size_t tokens, uint32_t top, const void *__restrict__ weights,
-                                                              int weight_elem, uint32_t dim, uint32_t chunks,
+                                                              int weight_elem, uint32_t dim, uint32_t chunks, uint32_t lanes,
                                                               T *__restrict__ grad_rows, void *__restrict__ grad_weights) {
-  const size_t t = (size_t)blockIdx.x * (kBlock / kWave) + wave_in_block();
+  typedef typename ChunkOf<T, VEC>::type chunk_t;
+  constexpr uint32_t U = 4, CH = 2;
+  __shared__ float wave_dot[WIDE ? kBlock / kWave : 1][U];
+  const uint32_t lane = threadIdx.x & (lanes - 1);
+  const size_t t = WIDE ? blockIdx.x : (size_t)blockIdx.x * (kBlock / lanes) + threadIdx.x / lanes;
   if (t >= tokens) return;
-  const uint32_t lane = lane_id(), n = (uint32_t)(tokens * top), n_live = (uint32_t)*live;
-  for (uint32_t k = 0; k < top; ++k) {
-    const uint32_t i = (uint32_t)t * top + k;
-    const uint32_t s = (uint32_t)slot[i];
-    const float w = weights ? load_weight(weights, weight_elem, i) : 1.f;
-    float dot = 0.f;
-    for (uint32_t c = lane; c < chunks; c += kWave) {
-      const uint32_t at = min(c * VEC, dim - VEC);
-      float g[VEC], v[VEC];
-      if (i >= n_live) {
+  const uint32_t n = (uint32_t)(tokens * top), n_live = (uint32_t)*live;
+  const T *from = grad_out + t * grad_stride;
+  for (uint32_t k0 = 0; k0 < top; k0 += U) {
+    const uint32_t i = (uint32_t)t * top + k0, last = min(U, top - k0) - 1;
+    uint32_t s[U];
+    float w[U], dot[U] = {};
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = 0.f;
-        store_chunk<T, VEC>(grad_rows + (size_t)i * dim + at, v);
-      }
-      if (s >= n) continue;
-      load_chunk<T, VEC>(grad_out + t * grad_stride + at, g);
-      if (grad_weights) {
-        load_chunk<T, VEC>(rows + s * stride + at, v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)  // an element that the chunk before has too is counted there
-          if (at + e >= c * VEC) dot = fmaf(v[e], g[e], dot);
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = w * g[e];
-      store_chunk<T, VEC>(grad_rows + (size_t)s * dim + at, v);
+    for (uint32_t u = 0; u < U; ++u) {
+      s[u] = u <= last ? (uint32_t)slot[i + u] : n;
+      w[u] = weights ? load_weight(weights, weight_elem, i + min(u, last)) : 1.f;
     }
-    if (grad_weights) {
+    for (uint32_t c0 = lane; c0 < chunks; c0 += lanes * CH) {
+      uint32_t at[CH];
+      chunk_t g[CH], v[U][CH];
 #pragma unroll
-      for (int d = kWave / 2; d > 0; d /= 2) dot += __shfl_xor(dot, d);
-      if (lane == 0) store_weight(grad_weights, weight_elem, i, dot);
+      for (uint32_t h = 0; h < CH; ++h) {
+        at[h] = min((c0 + h * lanes) * VEC, dim - VEC);
+        g[h] = raw_chunk<T, VEC>(from + at[h]);
+      }
+      if (grad_weights) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+          if (s[u] < n)
+#pragma unroll
+            for (uint32_t h = 0; h < CH; ++h) v[u][h] = raw_chunk<T, VEC, STREAM>(rows + s[u] * stride + at[h]);
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < CH; ++h) {
+        const uint32_t c = c0 + h * lanes;
+        if (c >= chunks) break;
+        float x[VEC];
+        to_floats<T, VEC>(g[h], x);
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+          if (i + u >= n_live && u <= last) put_chunk<T, VEC, STREAM>(grad_rows + (size_t)(i + u) * dim + at[h], chunk_t{});
+          if (s[u] >= n) continue;
+          float y[VEC];
+          if (grad_weights) {
+            to_floats<T, VEC>(v[u][h], y);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)  // an element that the chunk before has too is counted there
+              if (at[h] + e >= c * VEC) dot[u] = fmaf(y[e], x[e], dot[u]);
+          }
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) y[e] = w[u] * x[e];
+          store_chunk<T, VEC, STREAM>(grad_rows + (size_t)s[u] * dim + at[h], y);
+        }
+      }
+    }
+    if (!grad_weights) continue;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+      for (uint32_t d = min(lanes, (uint32_t)kWave) / 2; d > 0; d /= 2) dot[u] += __shfl_xor(dot[u], d);
+    if constexpr (WIDE) {
+      __syncthreads();  // the sums of the rows before have been read
+      if (lane_id() == 0)
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) wave_dot[wave_in_block()][u] = dot[u];
+      __syncthreads();
+      if (threadIdx.x <= last) {
+        float sum = 0.f;
+#pragma unroll
+        for (int q = 0; q < kBlock / kWave; ++q) sum += wave_dot[q][threadIdx.x];
+        store_weight(grad_weights, weight_elem, i + threadIdx.x, sum);
+      }
+    } else if (lane == 0) {
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+        if (u <= last) store_weight(grad_weights, weight_elem, i + u, dot[u]);
     }
   }
 }
@@ -171,13 +215,13 @@ int ugk_expert_dispatch(const void *x_dev, size_t x_stride, const int32_t *slot_
   if (int rc = check_rows("ugk_expert_dispatch", tokens, top, dim, elem, x_stride)) return rc;
   if (tokens == 0) return 0;
   UGK_REQUIRE(x_dev && slot_dev && live_dev && rows_dev, "ugk_expert_dispatch: null pointer");
-  return for_moved_rows(elem, dim, [&](auto type, auto vec) -> int {
+  return for_moved_rows(elem, dim, tokens * top, [&](auto type, auto vec, auto stream_out) -> int {
     typedef decltype(type) T;
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(tokens, s);
     UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_expert_dispatch: %zu tokens of %zu elements are more than one launch takes", tokens, dim);
-    hipLaunchKernelGGL((dispatch_kernel<T, V>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)x_dev, x_stride,
+    hipLaunchKernelGGL((dispatch_kernel<T, V, decltype(stream_out)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)x_dev, x_stride,
                        slot_dev, live_dev, tokens, top, (uint32_t)dim, s, (T *)rows_dev);
     UGK_HIP(hipGetLastError());
     return 0;
@@ -191,13 +235,13 @@ int ugk_expert_combine(const void *rows_dev, size_t n_rows, size_t row_stride, c
   UGK_REQUIRE(!weights_dev || elem_ok(weight_elem), "ugk_expert_combine: element code %d of the weights", weight_elem);
   if (tokens == 0) return 0;
   UGK_REQUIRE((rows_dev || n_rows == 0) && slot_dev && out_dev, "ugk_expert_combine: null pointer");
-  return for_rows(elem, dim, [&](auto type, auto vec) -> int {
+  return for_rows_streamed(elem, dim, n_rows, [&](auto type, auto vec, auto stream_rows) -> int {
     typedef decltype(type) T;
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(tokens, s);
     UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_expert_combine: %zu tokens of %zu elements are more than one launch takes", tokens, dim);
-    hipLaunchKernelGGL((combine_kernel<T, V>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)rows_dev, row_stride,
+    hipLaunchKernelGGL((combine_kernel<T, V, decltype(stream_rows)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)rows_dev, row_stride,
                        (uint32_t)n_rows, slot_dev, tokens, top, weights_dev, weight_elem, (uint32_t)dim, s, (T *)out_dev);
     UGK_HIP(hipGetLastError());
     return 0;
@@ -213,15 +257,25 @@ int ugk_expert_combine_grad(const void *grad_out_dev, size_t grad_stride, const 
   UGK_REQUIRE((!weights_dev && !grad_weights_dev) || elem_ok(weight_elem), "ugk_expert_combine_grad: element code %d of the weights", weight_elem);
   if (tokens == 0) return 0;
   UGK_REQUIRE(grad_out_dev && slot_dev && live_dev && grad_rows_dev && (rows_dev || !grad_weights_dev), "ugk_expert_combine_grad: null pointer");
-  return for_rows(elem, dim, [&](auto type, auto vec) -> int {
+  return for_rows_streamed(elem, dim, tokens * top, [&](auto type, auto vec, auto stream_rows) -> int {
     typedef decltype(type) T;
     constexpr int V = decltype(vec)::value;
-    constexpr int kPer = kBlock / kWave;
-    hipLaunchKernelGGL((combine_grad_kernel<T, V>), dim3((unsigned)((tokens + kPer - 1) / kPer)), dim3(kBlock), 0, as_stream(stream),
-                       (const T *)grad_out_dev, grad_stride, (const T *)rows_dev, row_stride, slot_dev, live_dev, tokens, top, weights_dev,
-                       weight_elem, (uint32_t)dim, split_of(dim, V).chunks, (T *)grad_rows_dev, grad_weights_dev);
-    UGK_HIP(hipGetLastError());
-    return 0;
+    constexpr bool S = decltype(stream_rows)::value;
+    const uint32_t chunks = split_of(dim, V).chunks;
+    uint32_t lanes = 4;
+    while (lanes < chunks && lanes < (uint32_t)kWave) lanes *= 2;
+    // a workgroup per token from 256 chunks on (us, both gradients of K rows of a token and the sum: 16,384 x 8 x 256 chunks 317
+    // against 335 with a wavefront per token; 4,099 x 3 x 251 chunks 33.5 against 32.4, 4,096 x 8 x 128 chunks 49 against 40)
+    const bool wide = chunks >= (uint32_t)kBlock;
+    const auto launch = [&](auto is_wide, size_t blocks, uint32_t of) -> int {
+      hipLaunchKernelGGL((combine_grad_kernel<T, V, S, decltype(is_wide)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),
+                         (const T *)grad_out_dev, grad_stride, (const T *)rows_dev, row_stride, slot_dev, live_dev, tokens, top, weights_dev,
+                         weight_elem, (uint32_t)dim, chunks, of, (T *)grad_rows_dev, grad_weights_dev);
+      UGK_HIP(hipGetLastError());
+      return 0;
+    };
+    const size_t per = kBlock / lanes;
+    return wide ? launch(std::true_type(), tokens, kBlock) : launch(std::false_type(), (tokens + per - 1) / per, lanes);
   });
 }
 

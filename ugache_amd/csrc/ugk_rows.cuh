@@ -27,9 +27,18 @@ struct ChunkOf<T, 1> {
   typedef T type;
 };
 
-template <typename T, int VEC>
+// STREAM: past the caches (non-temporal), for what is read once or written to be read much later
+template <typename T, int VEC, bool STREAM = false>
 __device__ __forceinline__ typename ChunkOf<T, VEC>::type raw_chunk(const T *from) {
-  return *reinterpret_cast<const typename ChunkOf<T, VEC>::type *>(from);
+  const typename ChunkOf<T, VEC>::type *p = reinterpret_cast<const typename ChunkOf<T, VEC>::type *>(from);
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <typename T, int VEC, bool STREAM = false>
+__device__ __forceinline__ void put_chunk(T *to, const typename ChunkOf<T, VEC>::type &v) {
+  typename ChunkOf<T, VEC>::type *p = reinterpret_cast<typename ChunkOf<T, VEC>::type *>(to);
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void to_floats(const typename ChunkOf<T, VEC>::type &v, float (&x)[VEC]) {
@@ -40,13 +49,12 @@ __device__ __forceinline__ void to_floats(const typename ChunkOf<T, VEC>::type &
     for (int i = 0; i < VEC; ++i) x[i] = (float)v[i];
   }
 }
-
 template <typename T, int VEC>
 __device__ __forceinline__ void load_chunk(const T *from, float (&x)[VEC]) {
   to_floats<T, VEC>(raw_chunk<T, VEC>(from), x);
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool STREAM = false>
 __device__ __forceinline__ void store_chunk(T *to, const float (&x)[VEC]) {
   typename ChunkOf<T, VEC>::type v;
   if constexpr (VEC == 1) {
@@ -55,7 +63,7 @@ __device__ __forceinline__ void store_chunk(T *to, const float (&x)[VEC]) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] = (T)x[i];
   }
-  *reinterpret_cast<typename ChunkOf<T, VEC>::type *>(to) = v;
+  put_chunk<T, VEC, STREAM>(to, v);
 }
 
 // a weight of any of the three types (a branch that the whole launch takes the same way)
@@ -100,11 +108,22 @@ static inline int for_rows(int elem, size_t dim, F f) {
   if (elem == 2) return dim >= 8 ? f(half_t(), std::integral_constant<int, 8>()) : f(half_t(), std::integral_constant<int, 1>());
   return dim >= 8 ? f(bhalf_t(), std::integral_constant<int, 8>()) : f(bhalf_t(), std::integral_constant<int, 1>());
 }
-// ... for kernels that move elements of two or four bytes without looking at them
+// ... and whether so many of them are more than the memory-side cache holds
 template <typename F>
-static inline int for_moved_rows(int elem, size_t dim, F f) {
-  if (elem == 4) return dim >= 4 ? f(uint32_t(), std::integral_constant<int, 4>()) : f(uint32_t(), std::integral_constant<int, 1>());
-  return dim >= 8 ? f(uint16_t(), std::integral_constant<int, 8>()) : f(uint16_t(), std::integral_constant<int, 1>());
+static inline int for_rows_streamed(int elem, size_t dim, size_t rows, F f) {
+  return for_rows(elem, dim, [&](auto type, auto vec) -> int {
+    return rows * dim * sizeof(type) > kMemorySideCacheBytes ? f(type, vec, std::true_type()) : f(type, vec, std::false_type());
+  });
+}
+// ... for kernels that move elements of two or four bytes without looking at them, and whether their output of so many rows is
+// stored past the caches
+template <typename F>
+static inline int for_moved_rows(int elem, size_t dim, size_t out_rows, F f) {
+  const auto stored = [&](auto type, auto vec) -> int {
+    return nt_store_for(out_rows * dim * sizeof(type)) ? f(type, vec, std::true_type()) : f(type, vec, std::false_type());
+  };
+  if (elem == 4) return dim >= 4 ? stored(uint32_t(), std::integral_constant<int, 4>()) : stored(uint32_t(), std::integral_constant<int, 1>());
+  return dim >= 8 ? stored(uint16_t(), std::integral_constant<int, 8>()) : stored(uint16_t(), std::integral_constant<int, 1>());
 }
 
 static inline bool elem_ok(int elem) { return elem == 4 || elem == 2 || elem == UGK_ELEM_BF16; }

@@ -12,19 +12,18 @@ namespace ugk {
 namespace {
 
 // out[i] = table[index[i]], a zero row where the index is outside [0, rows)
-template <typename T, int VEC, typename I>
+template <typename T, int VEC, bool STREAM, typename I>
 __global__ __launch_bounds__(kBlock) void take_rows_kernel(const T *__restrict__ table, uint64_t rows, size_t stride, const I *__restrict__ index,
                                                            size_t n, uint32_t dim, Split split, T *__restrict__ out) {
-  typedef typename ChunkOf<T, VEC>::type chunk_t;
   size_t i;
   uint32_t c;
   split_lane(split, blockIdx.x, i, c);
   if (i >= n) return;
   const uint32_t at = min(c * VEC, dim - VEC);
   const long long r = (long long)index[i];
-  chunk_t v = {};
-  if (r >= 0 && (uint64_t)r < rows) v = *reinterpret_cast<const chunk_t *>(table + (size_t)r * stride + at);
-  *reinterpret_cast<chunk_t *>(out + i * dim + at) = v;
+  typename ChunkOf<T, VEC>::type v = {};
+  if (r >= 0 && (uint64_t)r < rows) v = raw_chunk<T, VEC>(table + (size_t)r * stride + at);
+  put_chunk<T, VEC, STREAM>(out + i * dim + at, v);
 }
 
 // begin[r] = number of sorted keys below r, r = 0 .. rows.  A search per row, so that neither a run of rows nobody named nor a
@@ -72,7 +71,7 @@ constexpr uint32_t kPiece = 64;
 
 // out[r] = sum of the rows grad[entries[j]], begin[r] <= j < begin[r + 1], in fp32 in the order of j.  The first row_blocks
 // workgroups take the rows of at most kPiece entries, the others the pieces.
-template <typename T, int VEC>
+template <typename T, int VEC, bool STREAM>
 __global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ grad, size_t stride, const uint32_t *__restrict__ entries,
                                                          const uint32_t *__restrict__ keys, const uint32_t *__restrict__ begin,
                                                          uint32_t rows, uint32_t dim, Split split, uint32_t row_blocks, T *__restrict__ out,
@@ -88,7 +87,7 @@ __global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ g
     const uint32_t from = begin[i], to = begin[i + 1];
     if (to - from > kPiece) return;
     add_entries<T, VEC>(grad, stride, entries, from, to, at, sum);
-    store_chunk<T, VEC>(out + i * dim + at, sum);
+    store_chunk<T, VEC, STREAM>(out + i * dim + at, sum);
     return;
   }
   const uint32_t live = begin[rows];
@@ -167,13 +166,13 @@ int take_rows(const void *table, uint64_t num_rows, size_t stride, const I *inde
   UGK_REQUIRE(n < ((size_t)1 << 40) && num_rows < ((uint64_t)1 << 40), "ugk_take_rows: %zu of %zu rows", n, (size_t)num_rows);
   if (n == 0) return 0;
   UGK_REQUIRE((table || num_rows == 0) && index && out, "ugk_take_rows: null pointer");
-  return for_moved_rows(elem, dim, [&](auto type, auto vec) -> int {
+  return for_moved_rows(elem, dim, n, [&](auto type, auto vec, auto stream_out) -> int {
     typedef decltype(type) T;
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(n, s);
     UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_take_rows: %zu rows of %zu elements are more than one launch takes", n, dim);
-    hipLaunchKernelGGL((take_rows_kernel<T, V, I>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)table, num_rows,
+    hipLaunchKernelGGL((take_rows_kernel<T, V, decltype(stream_out)::value, I>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)table, num_rows,
                        stride, index, n, (uint32_t)dim, s, (T *)out);
     UGK_HIP(hipGetLastError());
     return 0;
@@ -221,7 +220,7 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
   }
   hipLaunchKernelGGL(row_begin_kernel, dim3((unsigned)(num_rows / kBlock + 1)), dim3(kBlock), 0, as_stream(stream), key[at], (uint32_t)n,
                      (uint32_t)num_rows, begin);
-  return for_rows(elem, dim, [&](auto type, auto vec) -> int {
+  return for_rows_streamed(elem, dim, num_rows, [&](auto type, auto vec, auto stream_out) -> int {
     typedef decltype(type) T;
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
@@ -229,7 +228,7 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
     const size_t row_blocks = split_blocks(num_rows, s), blocks = row_blocks + split_blocks(pieces, s);
     uint32_t lanes = 1;
     while (lanes < s.chunks && lanes < 32) lanes *= 2;
-    hipLaunchKernelGGL((row_sum_kernel<T, V>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)grad, stride, entry[at],
+    hipLaunchKernelGGL((row_sum_kernel<T, V, decltype(stream_out)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)grad, stride, entry[at],
                        key[at], begin, (uint32_t)num_rows, (uint32_t)dim, s, (uint32_t)row_blocks, (T *)out, parts);
     if (pieces > 0)
       hipLaunchKernelGGL((row_join_kernel<T, V>), dim3((unsigned)pieces, (s.chunks + lanes - 1) / lanes), dim3(kBlock), 0, as_stream(stream),
