@@ -464,6 +464,18 @@ def test_norm_and_clipping(name):
             assert all(torch.equal(a, b) for a, b in zip(again, grads))
 
 
+def test_norm_of_more_than_the_memory_side_cache_holds():
+    g = gen(35)
+    grads = [randn(g, 100_000_003, dtype=torch.bfloat16), randn(g, 60_000_001), randn(g, 5)]
+    out = [torch.empty_like(t) for t in grads]
+    check_norm(co.coll_torch_clip_grad_norm(grads, 3.0, out=out), grads)
+    check_clipped(out, grads, 3.0)
+    before = [t.clone() for t in grads]
+    co.coll_torch_clip_grad_norm(grads, 3.0)
+    assert all(torch.equal(a, b) for a, b in zip(grads, out))
+    check_clipped(grads, before, 3.0)
+
+
 @pytest.mark.parametrize("shift", [1, 2, 3, 5])
 def test_norm_at_odd_addresses(shift):
     g = gen(32)

@@ -3,6 +3,8 @@
 // norm = sqrt(sum over tensors and elements of x^2).  Squares and sums are held in 64 bits: a float's square needs twice
 // its exponent, and a thousand million terms need more than 24 bits.  Every workgroup sums one piece of one tensor, the
 // pieces' sums are added in their order, so the same gradients give the same bits on every run.
+#include <algorithm>
+
 #include "ugk_rows.cuh"
 
 namespace ugk {
@@ -42,7 +44,7 @@ __device__ __forceinline__ uint32_t tensor_of(const TensorList &list, uint32_t p
 
 // f for the 16-byte chunks of a piece, all of a lane's on their way at once where the piece is a whole one, and for the
 // elements behind the last chunk
-template <typename T, typename F>
+template <typename T, bool STREAM, typename F>
 __device__ __forceinline__ void for_elements(const T *data, uint64_t count, uint32_t piece, F f) {
   constexpr int VEC = 16 / sizeof(T), U = kPieceBytes / (16 * kBlock);
   constexpr uint32_t kElems = kPieceBytes / sizeof(T);
@@ -56,7 +58,7 @@ __device__ __forceinline__ void for_elements(const T *data, uint64_t count, uint
   if (whole) {
     typename ChunkOf<T, VEC>::type v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = raw_chunk<T, VEC>(from + (u * kBlock + threadIdx.x) * VEC);
+    for (int u = 0; u < U; ++u) v[u] = raw_chunk<T, VEC, STREAM>(from + (u * kBlock + threadIdx.x) * VEC);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float x[VEC];
@@ -91,22 +93,34 @@ __device__ __forceinline__ double block_sum(double v) {
   return sum;
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __device__ __forceinline__ double squares(const void *data, uint64_t count, uint32_t piece) {
   double sum = 0;
-  for_elements<T>(static_cast<const T *>(data), count, piece, [&](uint64_t, const auto &x, auto vec) {
+  for_elements<T, STREAM>(static_cast<const T *>(data), count, piece, [&](uint64_t, const auto &x, auto vec) {
 #pragma unroll
     for (int e = 0; e < decltype(vec)::value; ++e) sum = fma((double)x[e], (double)x[e], sum);
   });
   return sum;
 }
 
-__global__ __launch_bounds__(kBlock) void grad_squares_kernel(TensorList list, double *__restrict__ sums) {
+template <bool STREAM>
+__device__ __forceinline__ double squares_of(const Listed &t, uint32_t piece) {
+  return t.elem == 4   ? squares<float, STREAM>(t.data, t.count, piece)
+         : t.elem == 2 ? squares<half_t, STREAM>(t.data, t.count, piece)
+                       : squares<bhalf_t, STREAM>(t.data, t.count, piece);
+}
+
+// What the memory-side cache keeps between the two passes over the gradients: the last kKept pieces (224 MiB) are read for
+// the norm the ordinary way, the ones before them past the caches, and the second pass goes from the last piece to the first;
+// its stores go past the caches too where gradients and outputs are more than the cache holds.  us, norm and scaling into
+// other tensors, all ordinary / these rules: 1.4 GB of bfloat16 766 / 702, 302 MB 173 / 138, 151 MB 76 / 72.
+constexpr uint64_t kKept = ((uint64_t)224 << 20) / kPieceBytes;
+
+// the first `streamed` pieces past the caches
+__global__ __launch_bounds__(kBlock) void grad_squares_kernel(TensorList list, uint32_t streamed, double *__restrict__ sums) {
   const uint32_t at = tensor_of(list, blockIdx.x), piece = blockIdx.x - list.first[at];
   const Listed t = list.tensor[at];
-  const double mine = t.elem == 4   ? squares<float>(t.data, t.count, piece)
-                      : t.elem == 2 ? squares<half_t>(t.data, t.count, piece)
-                                    : squares<bhalf_t>(t.data, t.count, piece);
+  const double mine = blockIdx.x < streamed ? squares_of<true>(t, piece) : squares_of<false>(t, piece);
   const double sum = block_sum<kBlock>(mine);
   if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
@@ -131,20 +145,28 @@ __global__ __launch_bounds__(kNormBlock) void grad_norm_kernel(const double *__r
   }
 }
 
-template <typename T>
+template <typename T, bool STREAM, bool STREAM_OUT>
 __device__ __forceinline__ void scaled(const void *data, void *out, uint64_t count, uint32_t piece, float factor, float after) {
-  for_elements<T>(static_cast<const T *>(data), count, piece, [&](uint64_t at, const auto &x, auto vec) {
+  for_elements<T, STREAM>(static_cast<const T *>(data), count, piece, [&](uint64_t at, const auto &x, auto vec) {
     constexpr int VEC = decltype(vec)::value;
     float y[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) y[e] = x[e] * factor * after;
-    store_chunk<T, VEC>(static_cast<T *>(out) + at, y);
+    store_chunk<T, VEC, STREAM_OUT>(static_cast<T *>(out) + at, y);
   });
+}
+template <bool STREAM, bool STREAM_OUT>
+__device__ __forceinline__ void scale_one(const Listed &t, uint32_t piece, float factor, float after) {
+  if (t.elem == 4) scaled<float, STREAM, STREAM_OUT>(t.data, t.out, t.count, piece, factor, after);
+  else if (t.elem == 2) scaled<half_t, STREAM, STREAM_OUT>(t.data, t.out, t.count, piece, factor, after);
+  else scaled<bhalf_t, STREAM, STREAM_OUT>(t.data, t.out, t.count, piece, factor, after);
 }
 
 // out = data * min(1, max_norm / (norm + 1e-6)), rounded once; nothing to do in place where the factor is 1.  A norm that is
 // no number makes every element none.
-__global__ __launch_bounds__(kBlock) void grad_scale_kernel(TensorList list, const double *__restrict__ total, double max_norm) {
+// The first `kept` pieces are read the ordinary way.
+template <bool STREAM_OUT>
+__global__ __launch_bounds__(kBlock) void grad_scale_kernel(TensorList list, uint32_t kept, const double *__restrict__ total, double max_norm) {
   const double ratio = max_norm / (sqrt(*total) + 1e-6);
   // a factor near the end of float's range, which a norm beyond it brings, would lose its digits: it is multiplied in two steps
   const bool small = ratio < 0x1p-100;
@@ -155,9 +177,8 @@ __global__ __launch_bounds__(kBlock) void grad_scale_kernel(TensorList list, con
   const Listed t = list.tensor[at];
   const uint32_t piece = pieces_of(t.count, t.elem) - 1 - (blockIdx.x - list.first[at]);
   if (factor == 1.f && t.out == t.data) return;
-  if (t.elem == 4) scaled<float>(t.data, t.out, t.count, piece, factor, after);
-  else if (t.elem == 2) scaled<half_t>(t.data, t.out, t.count, piece, factor, after);
-  else scaled<bhalf_t>(t.data, t.out, t.count, piece, factor, after);
+  if (blockIdx.x < kept) scale_one<false, STREAM_OUT>(t, piece, factor, after);
+  else scale_one<true, STREAM_OUT>(t, piece, factor, after);
 }
 
 __global__ void preload_grad_norm_kernel() {}
@@ -209,7 +230,10 @@ int grad_norm(const char *what, const ugk_tensor_t *tensors, size_t n, void *wor
               (size_t)(pieces + 1) * sizeof(double));
   double *total = static_cast<double *>(workspace), *sums = total + 1;
   const int rc = for_lists(tensors, n, false, [&](const TensorList &list, uint64_t before) -> int {
-    hipLaunchKernelGGL(grad_squares_kernel, dim3(list.pieces), dim3(kBlock), 0, stream, list, sums + before);
+    // pieces in front of the last kKept of all
+    const uint64_t streamed = pieces > kKept + before ? pieces - kKept - before : 0;
+    hipLaunchKernelGGL(grad_squares_kernel, dim3(list.pieces), dim3(kBlock), 0, stream, list, (uint32_t)std::min<uint64_t>(streamed, list.pieces),
+                       sums + before);
     UGK_HIP(hipGetLastError());
     return 0;
   });
@@ -240,9 +264,20 @@ int ugk_grad_clip(const ugk_tensor_t *tensors, size_t n, double max_norm, void *
                   void *stream) {
   UGK_REQUIRE(max_norm >= 0, "ugk_grad_clip: a limit of %g", max_norm);
   if (int rc = grad_norm("ugk_grad_clip", tensors, n, workspace_dev, workspace_bytes, norm_dev, as_stream(stream))) return rc;
-  return for_lists(tensors, n, true, [&](const TensorList &list, uint64_t) -> int {
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(list.pieces), dim3(kBlock), 0, as_stream(stream), list,
-                       static_cast<const double *>(workspace_dev), max_norm);
+  uint64_t read = 0, written = 0;  // bytes
+  for (size_t i = 0; i < n; ++i) {
+    read += tensors[i].count * elem_size(tensors[i].elem);
+    if (tensors[i].out && tensors[i].out != tensors[i].data) written += tensors[i].count * elem_size(tensors[i].elem);
+  }
+  const bool stream_out = nt_store_for(read + written);
+  return for_lists(tensors, n, true, [&](const TensorList &list, uint64_t before) -> int {
+    const uint32_t kept = before < kKept ? (uint32_t)(kKept - before) : 0;
+    if (stream_out)
+      hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(list.pieces), dim3(kBlock), 0, as_stream(stream), list, kept,
+                         static_cast<const double *>(workspace_dev), max_norm);
+    else
+      hipLaunchKernelGGL(grad_scale_kernel<false>, dim3(list.pieces), dim3(kBlock), 0, as_stream(stream), list, kept,
+                         static_cast<const double *>(workspace_dev), max_norm);
     UGK_HIP(hipGetLastError());
     return 0;
   });
