@@ -179,7 +179,7 @@ int expert_sort(const K *ids, size_t n, uint32_t num_experts, int32_t *slot, int
               need);
   const Digits d{0, 0, 0, num_experts, bits_for(num_experts)};
   return sort_pass<kExperts, K>(ids, nullptr, n, d, static_cast<uint32_t *>(workspace), reinterpret_cast<uint32_t *>(slot),
-                                reinterpret_cast<uint32_t *>(src), reinterpret_cast<uint32_t *>(offsets), as_stream(stream));
+                                reinterpret_cast<uint32_t *>(src), reinterpret_cast<uint32_t *>(offsets), nullptr, 1, as_stream(stream));
 }
 
 // what the entry points that move rows ask of their sizes

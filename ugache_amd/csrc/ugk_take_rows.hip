@@ -26,55 +26,123 @@ __global__ __launch_bounds__(kBlock) void take_rows_kernel(const T *__restrict__
   put_chunk<T, VEC, STREAM>(out + i * dim + at, v);
 }
 
-// begin[r] = number of sorted keys below r, r = 0 .. rows.  A search per row, so that neither a run of rows nobody named nor a
-// row everybody named is one lane's work; neighbouring rows walk the same way, a request for a wavefront.
-__global__ __launch_bounds__(kBlock) void row_begin_kernel(const uint32_t *__restrict__ keys, uint32_t n, uint32_t rows,
-                                                           uint32_t *__restrict__ begin) {
-  const uint32_t r = blockIdx.x * kBlock + threadIdx.x;
-  if (r > rows) return;
-  uint32_t lo = 0, hi = n;
+// the first position in [lo, hi) whose key is not below r; hi if there is none
+__device__ __forceinline__ uint32_t first_of(const uint32_t *keys, uint32_t lo, uint32_t hi, uint32_t r) {
   while (lo < hi) {
     const uint32_t mid = lo + (hi - lo) / 2;
     if (keys[mid] < r) lo = mid + 1;
     else hi = mid;
   }
-  begin[r] = lo;
+  return lo;
+}
+// the same for a wavefront that searches for one row: 64 keys a step
+__device__ __forceinline__ uint32_t wave_first_of(const uint32_t *keys, uint32_t lo, uint32_t hi, uint32_t r) {
+  while (hi > lo) {
+    const uint32_t step = (hi - lo + kWave - 1) / kWave, at = lo + lane_id() * step;
+    const uint32_t less = (uint32_t)__popcll(__ballot(at < hi && keys[min(at, hi - 1)] < r));  // they come first
+    if (step == 1) return lo + less;
+    hi = min(lo + less * step, hi);
+    lo = less ? lo + (less - 1) * step + 1 : lo;
+  }
+  return lo;
+}
+
+// begin[r] = number of sorted keys below r, r = 0 .. rows.  A search per row, so that neither a run of rows nobody named nor a
+// row everybody named is one lane's work: wavefronts find the workgroup's first and last row among all keys, its lanes
+// theirs between the two.
+__global__ __launch_bounds__(kBlock) void row_begin_kernel(const uint32_t *__restrict__ keys, uint32_t n, uint32_t rows,
+                                                           uint32_t *__restrict__ begin) {
+  __shared__ uint32_t ends[2];
+  const uint32_t r0 = blockIdx.x * kBlock, r = r0 + threadIdx.x, wave = wave_in_block();
+  if (wave < 2) {
+    const uint32_t found = wave_first_of(keys, 0, n, wave == 0 ? r0 : min(r0 + kBlock, rows));
+    if (lane_id() == 0) ends[wave] = found;
+  }
+  __syncthreads();
+  if (r <= rows) begin[r] = first_of(keys, ends[0], ends[1], r);
 }
 
 // sum += the rows grad[entries[j]], from <= j < to, in the order of j
 template <typename T, int VEC>
 __device__ __forceinline__ void add_entries(const T *grad, size_t stride, const uint32_t *entries, uint32_t from, uint32_t to, uint32_t at,
                                             float (&sum)[VEC]) {
-  constexpr int U = 4;  // rows on their way
+  constexpr uint32_t U = 4;  // rows on their way
   uint32_t j = from;
   for (; j + U <= to; j += U) {
-    float v[U][VEC];
+    typename ChunkOf<T, VEC>::type v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_chunk<T, VEC>(grad + (size_t)entries[j + u] * stride + at, v[u]);
+    for (uint32_t u = 0; u < U; ++u) v[u] = raw_chunk<T, VEC>(grad + (size_t)entries[j + u] * stride + at);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (uint32_t u = 0; u < U; ++u) {
+      float x[VEC];
+      to_floats<T, VEC>(v[u], x);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e] += v[u][e];
+      for (int e = 0; e < VEC; ++e) sum[e] += x[e];
+    }
   }
   for (; j < to; ++j) {
-    float v[VEC];
-    load_chunk<T, VEC>(grad + (size_t)entries[j] * stride + at, v);
+    float x[VEC];
+    load_chunk<T, VEC>(grad + (size_t)entries[j] * stride + at, x);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) sum[e] += v[e];
+    for (int e = 0; e < VEC; ++e) sum[e] += x[e];
   }
 }
 
-// A row of more than kPiece entries is summed in pieces: the positions are cut into pieces of kPiece, and a piece holds parts
-// of at most two such rows, one that comes in from the piece before and one that begins in it and goes on behind it.
-// parts[2 * piece] and parts[2 * piece + 1] are their sums.
-constexpr uint32_t kPiece = 64;
+// A row of more than `piece` entries is summed in pieces: the positions are cut into runs of `piece`, and a run holds parts of
+// at most two such rows, one that comes in from the run before and one that begins in it and goes on behind it.
+// parts[2 * run] and parts[2 * run + 1] are their sums.
+//
+// Where a row's entries are is in begin[] (BY_ROW), or is searched for among the keys.
+struct Sorted {
+  const uint32_t *keys, *begin;
+  uint32_t n, rows, piece;
+};
 
-// out[r] = sum of the rows grad[entries[j]], begin[r] <= j < begin[r + 1], in fp32 in the order of j.  The first row_blocks
-// workgroups take the rows of at most kPiece entries, the others the pieces.
-template <typename T, int VEC, bool STREAM>
+// whether a row that is summed in pieces begins in a run; the row, its first position, and where the run's entries end
+template <bool BY_ROW>
+__device__ __forceinline__ bool long_row_from(const Sorted &s, uint32_t run, uint32_t &row, uint32_t &first, uint32_t &to) {
+  const uint32_t from = run * s.piece;
+  if constexpr (BY_ROW) {
+    const uint32_t live = s.begin[s.rows];
+    if (from >= live) return false;
+    to = min(from + s.piece, live);
+    row = s.keys[to - 1];
+    first = s.begin[row];
+    return first >= from && s.begin[row + 1] - first > s.piece;
+  } else {
+    to = min(from + s.piece, s.n);
+    row = s.keys[to - 1];
+    // it goes on behind the run, and did not begin before it
+    if (row >= s.rows || to == s.n || s.keys[to] != row || (from > 0 && s.keys[from - 1] == row)) return false;
+    first = first_of(s.keys, from, to, row);
+    return first + s.piece < s.n && s.keys[first + s.piece] == row;
+  }
+}
+// whether a row that is summed in pieces comes into a run from the one before, and where its entries end there
+template <bool BY_ROW>
+__device__ __forceinline__ bool long_row_into(const Sorted &s, uint32_t run, uint32_t &end) {
+  const uint32_t from = run * s.piece, to = min(from + s.piece, s.n);
+  if (from >= s.n || from == 0) return false;
+  const uint32_t row = s.keys[from];
+  if (row >= s.rows) return false;
+  if constexpr (BY_ROW) {
+    const uint32_t first = s.begin[row], last = s.begin[row + 1];
+    end = min(to, last);
+    return first < from && last - first > s.piece;
+  } else {
+    if (s.keys[from - 1] != row) return false;
+    const uint32_t first = s.keys[from - s.piece] == row ? from - s.piece : first_of(s.keys, from - s.piece, from, row);
+    if (first + s.piece >= s.n || s.keys[first + s.piece] != row) return false;
+    end = s.keys[to - 1] == row ? to : first_of(s.keys, from, to, row + 1);
+    return true;
+  }
+}
+
+// The parts of the runs, and the rows of at most `piece` entries.  BY_ROW: a lane's row is i (the first row_blocks workgroups),
+// and one without entries is zero.  Otherwise i is a position, the lane's row the one that begins there, and out holds zeros.
+template <typename T, int VEC, bool BY_ROW, bool STREAM>
 __global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ grad, size_t stride, const uint32_t *__restrict__ entries,
-                                                         const uint32_t *__restrict__ keys, const uint32_t *__restrict__ begin,
-                                                         uint32_t rows, uint32_t dim, Split split, uint32_t row_blocks, T *__restrict__ out,
+                                                         Sorted s, uint32_t dim, Split split, uint32_t row_blocks, T *__restrict__ out,
                                                          float *__restrict__ parts) {
   size_t i;
   uint32_t c;
@@ -82,48 +150,54 @@ __global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ g
   split_lane(split, whole ? blockIdx.x : blockIdx.x - row_blocks, i, c);
   const uint32_t at = min(c * VEC, dim - VEC);
   float sum[VEC] = {};
+  uint32_t from, to;
   if (whole) {
-    if (i >= rows) return;
-    const uint32_t from = begin[i], to = begin[i + 1];
-    if (to - from > kPiece) return;
+    if constexpr (BY_ROW) {
+      if (i >= s.rows) return;
+      from = s.begin[i], to = s.begin[i + 1];
+      if (to - from > s.piece) return;
+    } else {
+      if (i >= s.n) return;
+      from = (uint32_t)i;
+      const uint32_t r = s.keys[from];
+      if (r >= s.rows || (from > 0 && s.keys[from - 1] == r)) return;
+      to = min(from + s.piece, s.n);
+      if (to < s.n && s.keys[to] == r) return;
+      to = from + 1 < s.n && s.keys[from + 1] == r ? first_of(s.keys, from + 2, to, r + 1) : from + 1;
+      i = r;
+    }
     add_entries<T, VEC>(grad, stride, entries, from, to, at, sum);
     store_chunk<T, VEC, STREAM>(out + i * dim + at, sum);
     return;
   }
-  const uint32_t live = begin[rows];
-  const uint32_t from = (uint32_t)i * kPiece;  // below n + kPiece
-  if (i * kPiece >= live) return;
-  const uint32_t to = min(from + kPiece, live);
-  const uint32_t r0 = keys[from], begin0 = begin[r0], end0 = begin[r0 + 1];
-  if (begin0 < from && end0 - begin0 > kPiece) {
-    add_entries<T, VEC>(grad, stride, entries, from, min(to, end0), at, sum);
+  if (i * s.piece >= s.n) return;
+  if (long_row_into<BY_ROW>(s, (uint32_t)i, to)) {
+    add_entries<T, VEC>(grad, stride, entries, (uint32_t)i * s.piece, to, at, sum);
     store_chunk<float, VEC>(parts + 2 * i * dim + at, sum);
   }
-  const uint32_t r1 = keys[to - 1], begin1 = begin[r1];
-  if (begin1 >= from && begin[r1 + 1] - begin1 > kPiece) {
+  uint32_t row;
+  if (long_row_from<BY_ROW>(s, (uint32_t)i, row, from, to)) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
-    add_entries<T, VEC>(grad, stride, entries, begin1, to, at, sum);
+    add_entries<T, VEC>(grad, stride, entries, from, to, at, sum);
     store_chunk<float, VEC>(parts + (2 * i + 1) * dim + at, sum);
   }
 }
 
-// The pieces of a row added up: a workgroup per piece in which such a row begins and per `lanes` chunks of it.  kBlock /
-// lanes groups of lanes add a run of the pieces each, then the groups' sums are added in their order.
-template <typename T, int VEC>
-__global__ __launch_bounds__(kBlock) void row_join_kernel(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ begin, uint32_t rows,
-                                                          uint32_t dim, uint32_t chunks, uint32_t lanes, const float *__restrict__ parts,
-                                                          T *__restrict__ out) {
+// The parts of a row added up: a workgroup per run in which such a row begins and per `lanes` chunks of it.  kBlock / lanes
+// groups of lanes add consecutive parts each, then the groups' sums are added in their order.
+template <typename T, int VEC, bool BY_ROW>
+__global__ __launch_bounds__(kBlock) void row_join_kernel(Sorted s, uint32_t dim, uint32_t chunks, uint32_t lanes,
+                                                          const float *__restrict__ parts, T *__restrict__ out) {
   __shared__ float held[kBlock * VEC];
-  const uint32_t live = begin[rows];
-  const uint32_t first = blockIdx.x * kPiece;  // below n
-  if (first >= live) return;
-  const uint32_t r = keys[min(first + kPiece, live) - 1], from = begin[r], to = begin[r + 1];
-  if (from < first || to - from <= kPiece) return;
+  uint32_t r, from, to;
+  if (!long_row_from<BY_ROW>(s, blockIdx.x, r, from, to)) return;
+  if constexpr (BY_ROW) to = s.begin[r + 1];
+  else to = wave_first_of(s.keys, to, s.n, r + 1);
   const uint32_t group = threadIdx.x / lanes, groups = kBlock / lanes;  // lanes: a power of two
   const uint32_t c = blockIdx.y * lanes + threadIdx.x % lanes;
   const uint32_t at = min(c * VEC, dim - VEC);
-  const uint32_t p0 = blockIdx.x, pieces = (to - 1) / kPiece - p0 + 1;
+  const uint32_t p0 = blockIdx.x, pieces = (to - 1) / s.piece - p0 + 1;
   const uint32_t per = (pieces + groups - 1) / groups;
   float sum[VEC] = {};
   if (c < chunks) {
@@ -151,6 +225,9 @@ __global__ __launch_bounds__(kBlock) void row_join_kernel(const uint32_t *__rest
     for (int e = 0; e < VEC; ++e) sum[e] += held[e * kBlock + g * lanes + threadIdx.x];
   store_chunk<T, VEC>(out + (size_t)r * dim + at, sum);
 }
+
+// more of the output than the sort's launches clear on their side
+__global__ __launch_bounds__(kSortBlock) void clear_kernel(Clear clear) { clear_block(clear, blockIdx.x); }
 
 __global__ void preload_take_rows_kernel() {}
 
@@ -189,7 +266,19 @@ Plan plan_for(uint64_t rows) {
   return Plan{passes, (bits + passes - 1) / passes};
 }
 
-size_t pieces_of(size_t n) { return (n + kPiece - 1) / kPiece; }
+// Where at least half of the rows are named by nobody the output is cleared on the side of the sort, which leaves the memory
+// idle, and only rows with entries are visited after it; where most are named that would store them twice.  us, by position /
+// by row: 16,384 entries over 50,000 bfloat16 rows of 2 KB 64 / 74, 100 over 3,000,000 of 32 bytes 19 / 40, 25,000 over 50,000 of
+// 2 KB 101 / 110, 30,000 105 / 104; 40,000 over 40,000 of 4 KB 156 / 113, 262,144 over 60,000 of 512 bytes 137 / 107.
+bool sums_by_row(size_t n, uint64_t rows) { return rows < 2 * (uint64_t)n; }
+
+// Entries a lane adds one after the other: few where the batch is small and their latency is what it costs, more where the
+// parts are traffic.  us, of 16 / 32 / 64: 16,384 bfloat16 rows of 1,024 elements 56 / 59 / 63, 30,000 95 / 95 / 104, 100,000 fp32
+// rows of 128 120 / 124 / 137, 262,144 of them 115 / 105 / 107, 30,000 bfloat16 rows of 2,048 132 / 126 / 132.
+uint32_t piece_for(size_t n, size_t dim) { return n * dim <= 20'000'000 ? 16u : 32u; }
+size_t pieces_of(size_t n, size_t dim) { return (n + piece_for(n, dim) - 1) / piece_for(n, dim); }
+
+size_t begin_words(size_t n, uint64_t rows) { return sums_by_row(n, rows) ? (size_t)rows + 1 : 0; }
 
 template <typename I>
 int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, uint64_t num_rows, size_t dim, int elem, void *out,
@@ -202,37 +291,68 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
   if (num_rows == 0) return 0;
   UGK_REQUIRE(out && (n == 0 || (grad && index)), "ugk_take_rows_grad: null pointer");
   const size_t need = ugk_take_rows_grad_workspace_bytes(n, num_rows, dim);
-  UGK_REQUIRE(workspace && workspace_bytes >= need, "ugk_take_rows_grad: a workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+  UGK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "ugk_take_rows_grad: a workspace of %zu bytes, %zu are needed", workspace_bytes, need);
   uint32_t *begin = static_cast<uint32_t *>(workspace);
-  uint32_t *key[2] = {begin + num_rows + 1, begin + num_rows + 1 + n}, *entry[2] = {key[1] + n, key[1] + 2 * n};
+  uint32_t *key[2] = {begin + begin_words(n, num_rows), begin + begin_words(n, num_rows) + n}, *entry[2] = {key[1] + n, key[1] + 2 * n};
   float *parts = reinterpret_cast<float *>(entry[1] + n);
-  uint32_t *words = reinterpret_cast<uint32_t *>(parts + 2 * pieces_of(n) * dim);
+  uint32_t *words = reinterpret_cast<uint32_t *>(parts + 2 * pieces_of(n, dim) * dim);
+  if (n == 0) {
+    Clearing all(out, num_rows * dim * elem_size(elem));
+    Clear clear;
+    const uint32_t blocks = all.take(clear, 1, 1);
+    hipLaunchKernelGGL(clear_kernel, dim3(blocks), dim3(kSortBlock), 0, as_stream(stream), clear);
+    UGK_HIP(hipGetLastError());
+    return 0;
+  }
   const Plan p = plan_for(num_rows);
+  const bool by_row = sums_by_row(n, num_rows);
+  Clearing clearing(out, by_row ? 0 : num_rows * dim * elem_size(elem));
+  Digits d{num_rows, 0, (1u << p.digit) - 1u, 1u << p.digit, p.digit};
   int at = 0;
-  if (n > 0) {
-    Digits d{num_rows, 0, (1u << p.digit) - 1u, 1u << p.digit, p.digit};
-    if (int rc = sort_pass<kFirst, I>(index, nullptr, n, d, words, key[0], entry[0], nullptr, as_stream(stream))) return rc;
+  const SortShape shape = sort_shape(n);
+  if (shape.reach == kSingle) {
+    Clear clear;
+    const uint32_t blocks = clearing.take(clear, 1, 1);
+    const auto one = [&](auto items) {
+      hipLaunchKernelGGL((sort_one_tile_kernel<I, decltype(items)::value>), dim3(1 + blocks), dim3(kSortBlock), 0, as_stream(stream), index,
+                         (uint32_t)n, p.passes, d, clear, key[0], entry[0]);
+    };
+    if (shape.items == 2) one(std::integral_constant<int, 2>());
+    else one(std::integral_constant<int, 8>());
+    UGK_HIP(hipGetLastError());
+  } else {
+    if (int rc = sort_pass<kFirst, I>(index, nullptr, n, d, words, key[0], entry[0], nullptr, &clearing, p.passes, as_stream(stream))) return rc;
     for (uint32_t pass = 1; pass < p.passes; ++pass, at ^= 1) {
       d.shift += p.digit;
-      if (int rc = sort_pass<kNext, uint32_t>(key[at], entry[at], n, d, words, key[at ^ 1], entry[at ^ 1], nullptr, as_stream(stream)))
+      if (int rc = sort_pass<kNext, uint32_t>(key[at], entry[at], n, d, words, key[at ^ 1], entry[at ^ 1], nullptr, &clearing, p.passes - pass,
+                                              as_stream(stream)))
         return rc;
     }
   }
-  hipLaunchKernelGGL(row_begin_kernel, dim3((unsigned)(num_rows / kBlock + 1)), dim3(kBlock), 0, as_stream(stream), key[at], (uint32_t)n,
-                     (uint32_t)num_rows, begin);
+  if (by_row)
+    hipLaunchKernelGGL(row_begin_kernel, dim3((unsigned)(num_rows / kBlock + 1)), dim3(kBlock), 0, as_stream(stream), key[at], (uint32_t)n,
+                       (uint32_t)num_rows, begin);
   return for_rows_streamed(elem, dim, num_rows, [&](auto type, auto vec, auto stream_out) -> int {
     typedef decltype(type) T;
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
-    const size_t pieces = n > kPiece ? pieces_of(n) : 0;  // in fewer entries no row has more than a piece
-    const size_t row_blocks = split_blocks(num_rows, s), blocks = row_blocks + split_blocks(pieces, s);
+    const uint32_t piece = piece_for(n, dim);
+    const Sorted sorted{key[at], begin, (uint32_t)n, (uint32_t)num_rows, piece};
+    const size_t pieces = n > piece ? pieces_of(n, dim) : 0;  // in fewer entries no row has more than a piece
+    const size_t row_blocks = split_blocks(by_row ? num_rows : n, s), blocks = row_blocks + split_blocks(pieces, s);
+    UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_take_rows_grad: %zu rows of %zu elements are more than one launch takes", (size_t)num_rows, dim);
     uint32_t lanes = 1;
     while (lanes < s.chunks && lanes < 32) lanes *= 2;
-    hipLaunchKernelGGL((row_sum_kernel<T, V, decltype(stream_out)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)grad, stride, entry[at],
-                       key[at], begin, (uint32_t)num_rows, (uint32_t)dim, s, (uint32_t)row_blocks, (T *)out, parts);
-    if (pieces > 0)
-      hipLaunchKernelGGL((row_join_kernel<T, V>), dim3((unsigned)pieces, (s.chunks + lanes - 1) / lanes), dim3(kBlock), 0, as_stream(stream),
-                         key[at], begin, (uint32_t)num_rows, (uint32_t)dim, s.chunks, lanes, parts, (T *)out);
+    const auto launch = [&](auto rowwise, auto stored) {
+      constexpr bool R = decltype(rowwise)::value;
+      hipLaunchKernelGGL((row_sum_kernel<T, V, R, decltype(stored)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),
+                         (const T *)grad, stride, entry[at], sorted, (uint32_t)dim, s, (uint32_t)row_blocks, (T *)out, parts);
+      if (pieces > 0)
+        hipLaunchKernelGGL((row_join_kernel<T, V, R>), dim3((unsigned)pieces, (s.chunks + lanes - 1) / lanes), dim3(kBlock), 0, as_stream(stream),
+                           sorted, (uint32_t)dim, s.chunks, lanes, parts, (T *)out);
+    };
+    if (by_row) launch(std::true_type(), stream_out);
+    else launch(std::false_type(), std::false_type());
     UGK_HIP(hipGetLastError());
     return 0;
   });
@@ -255,7 +375,7 @@ int ugk_take_rows_i64(const void *table_dev, uint64_t num_rows, size_t stride, c
 }
 
 size_t ugk_take_rows_grad_workspace_bytes(size_t n, uint64_t num_rows, size_t dim) {
-  return 4 * ((size_t)num_rows + 1 + 4 * n + 2 * pieces_of(n) * dim + sort_count_words(n, 1u << plan_for(num_rows).digit));
+  return 4 * (begin_words(n, num_rows) + 4 * n + 2 * pieces_of(n, dim) * dim + sort_count_words(n, 1u << plan_for(num_rows).digit));
 }
 int ugk_take_rows_grad_i32(const void *grad_dev, size_t stride, const int32_t *index_dev, size_t n, uint64_t num_rows, size_t dim, int elem,
                            void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream) {
