@@ -266,11 +266,13 @@ Plan plan_for(uint64_t rows) {
   return Plan{passes, (bits + passes - 1) / passes};
 }
 
-// Where at least half of the rows are named by nobody the output is cleared on the side of the sort, which leaves the memory
-// idle, and only rows with entries are visited after it; where most are named that would store them twice.  us, by position /
-// by row: 16,384 entries over 50,000 bfloat16 rows of 2 KB 64 / 74, 100 over 3,000,000 of 32 bytes 19 / 40, 25,000 over 50,000 of
-// 2 KB 101 / 110, 30,000 105 / 104; 40,000 over 40,000 of 4 KB 156 / 113, 262,144 over 60,000 of 512 bytes 137 / 107.
-bool sums_by_row(size_t n, uint64_t rows) { return rows < 2 * (uint64_t)n; }
+// Where some rows are named by nobody for certain the output is cleared on the side of the sort, which leaves the memory idle,
+// and only rows with entries are visited after it; where most may be named that would store them twice, but for outputs so
+// small that the launch which finds where rows begin costs more.  us, by position / by row: 16,384 entries over 50,000 bfloat16
+// rows of 2 KB 46 / 62, 40,000 over 50,000 76 / 98, 100,000 over 200,000 of 256 bytes 70 / 69; 3,000 over 3,000 of 128 bytes 18.6 /
+// 21.0, 10,000 over 5,000 of 256 bytes 30 / 31; 40,000 over 40,000 of 4 KB 145 / 111, 200,000 over 100,000 of 128 bytes 65 / 55,
+// 262,144 over 60,000 of 512 bytes 133 / 105.
+bool sums_by_row(size_t n, uint64_t rows, size_t dim) { return rows <= n && (n > 32768 || rows * dim > 4'000'000); }
 
 // Entries a lane adds one after the other: few where the batch is small and their latency is what it costs, more where the
 // parts are traffic.  us, of 16 / 32 / 64: 16,384 bfloat16 rows of 1,024 elements 56 / 59 / 63, 30,000 95 / 95 / 104, 100,000 fp32
@@ -278,7 +280,7 @@ bool sums_by_row(size_t n, uint64_t rows) { return rows < 2 * (uint64_t)n; }
 uint32_t piece_for(size_t n, size_t dim) { return n * dim <= 20'000'000 ? 16u : 32u; }
 size_t pieces_of(size_t n, size_t dim) { return (n + piece_for(n, dim) - 1) / piece_for(n, dim); }
 
-size_t begin_words(size_t n, uint64_t rows) { return sums_by_row(n, rows) ? (size_t)rows + 1 : 0; }
+size_t begin_words(size_t n, uint64_t rows, size_t dim) { return sums_by_row(n, rows, dim) ? (size_t)rows + 1 : 0; }
 
 template <typename I>
 int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, uint64_t num_rows, size_t dim, int elem, void *out,
@@ -293,7 +295,7 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
   const size_t need = ugk_take_rows_grad_workspace_bytes(n, num_rows, dim);
   UGK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "ugk_take_rows_grad: a workspace of %zu bytes, %zu are needed", workspace_bytes, need);
   uint32_t *begin = static_cast<uint32_t *>(workspace);
-  uint32_t *key[2] = {begin + begin_words(n, num_rows), begin + begin_words(n, num_rows) + n}, *entry[2] = {key[1] + n, key[1] + 2 * n};
+  uint32_t *key[2] = {begin + begin_words(n, num_rows, dim), begin + begin_words(n, num_rows, dim) + n}, *entry[2] = {key[1] + n, key[1] + 2 * n};
   float *parts = reinterpret_cast<float *>(entry[1] + n);
   uint32_t *words = reinterpret_cast<uint32_t *>(parts + 2 * pieces_of(n, dim) * dim);
   if (n == 0) {
@@ -305,7 +307,7 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
     return 0;
   }
   const Plan p = plan_for(num_rows);
-  const bool by_row = sums_by_row(n, num_rows);
+  const bool by_row = sums_by_row(n, num_rows, dim);
   Clearing clearing(out, by_row ? 0 : num_rows * dim * elem_size(elem));
   Digits d{num_rows, 0, (1u << p.digit) - 1u, 1u << p.digit, p.digit};
   int at = 0;
@@ -375,7 +377,7 @@ int ugk_take_rows_i64(const void *table_dev, uint64_t num_rows, size_t stride, c
 }
 
 size_t ugk_take_rows_grad_workspace_bytes(size_t n, uint64_t num_rows, size_t dim) {
-  return 4 * (begin_words(n, num_rows) + 4 * n + 2 * pieces_of(n, dim) * dim + sort_count_words(n, 1u << plan_for(num_rows).digit));
+  return 4 * (begin_words(n, num_rows, dim) + 4 * n + 2 * pieces_of(n, dim) * dim + sort_count_words(n, 1u << plan_for(num_rows).digit));
 }
 int ugk_take_rows_grad_i32(const void *grad_dev, size_t stride, const int32_t *index_dev, size_t n, uint64_t num_rows, size_t dim, int elem,
                            void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream) {
