@@ -357,23 +357,28 @@ static inline uint32_t bits_for(uint64_t values) {  // that tell `values` number
   while (((uint64_t)1 << bits) < values) ++bits;
   return bits;
 }
-// How a pass goes by its size.
+// How a pass goes by its size.  Small tiles spread a batch over the chip, large ones keep the counts of all tiles few.  us of a
+// sort, entries per lane 2 / 4 / 8: 96,000 entries in 64 buckets 10.5 / 11.2 / 14.4, 480,000 11.6 / 11.9 / 15.1, 480,000 in 1,000
+// 23.0 / 18.7 / 20.3, 1 M in 128 18.1 / 15.8 / 17.2, two passes of 1 M over 1,024 124 / 107 / 97; 32,000 in 64, counts of the
+// tiles added up by every workgroup / by a launch of their own 8.5 / 10.5, 64,000 10.3 / 10.4.
 struct SortShape {
   int items;
   Reach reach;
   uint32_t tiles;
 };
-static inline SortShape sort_shape(size_t n) {
+static inline SortShape sort_shape(size_t n, uint32_t buckets) {
   const auto tiles = [n](int items) { return (uint32_t)((n + kSortBlock * items - 1) / (kSortBlock * items)); };
   if (n <= 2 * kSortBlock) return SortShape{2, kSingle, 1};
+  if (n <= 4 * kSortBlock) return SortShape{4, kSingle, 1};
   if (n <= 8 * kSortBlock) return SortShape{8, kSingle, 1};
-  if (tiles(2) <= 16) return SortShape{2, kFew, tiles(2)};
-  if (tiles(8) <= 32) return SortShape{8, kFew, tiles(8)};
+  if (tiles(2) <= 32) return SortShape{2, kFew, tiles(2)};
+  if ((uint64_t)tiles(2) * buckets <= 100'000) return SortShape{2, kMany, tiles(2)};
+  if ((uint64_t)tiles(4) * buckets <= 250'000) return SortShape{4, kMany, tiles(4)};
   return SortShape{8, kMany, tiles(8)};
 }
 // words of the counts of a pass: of every tile, summed over the tiles before, and of all
 static inline size_t sort_count_words(size_t n, uint32_t buckets) {
-  const SortShape s = sort_shape(n);
+  const SortShape s = sort_shape(n, buckets);
   return s.reach == kSingle ? 0 : s.reach == kFew ? (size_t)s.tiles * buckets : (2 * (size_t)s.tiles + 1) * buckets;
 }
 
@@ -417,19 +422,20 @@ static inline int sort_pass_as(const K *keys, const uint32_t *entries, size_t n,
 template <Pass P, typename K>
 static inline int sort_pass(const K *keys, const uint32_t *entries, size_t n, const Digits &d, uint32_t *words, uint32_t *out0,
                             uint32_t *out1, uint32_t *offsets, Clearing *clearing, uint32_t passes_left, hipStream_t stream) {
-  const SortShape s = sort_shape(n);
+  const SortShape s = sort_shape(n, d.buckets);
   const auto as = [&](auto items, auto reach) -> int {
     return sort_pass_as<P, K, decltype(items)::value, decltype(reach)::value>(keys, entries, n, d, s.tiles, words, out0, out1, offsets, clearing,
                                                                              passes_left, stream);
   };
   const std::integral_constant<int, 2> two;
+  const std::integral_constant<int, 4> four;
   const std::integral_constant<int, 8> eight;
-  if (s.reach == kMany) return as(eight, std::integral_constant<Reach, kMany>());
-  if (s.reach == kFew && s.items == 8) return as(eight, std::integral_constant<Reach, kFew>());
+  const std::integral_constant<Reach, kMany> many;
+  if (s.reach == kMany) return s.items == 2 ? as(two, many) : s.items == 4 ? as(four, many) : as(eight, many);
   if (s.reach == kFew) return as(two, std::integral_constant<Reach, kFew>());
   if constexpr (P == kExperts) {  // the others sort one tile by sort_one_tile_kernel
-    if (s.items == 8) return as(eight, std::integral_constant<Reach, kSingle>());
-    return as(two, std::integral_constant<Reach, kSingle>());
+    const std::integral_constant<Reach, kSingle> single;
+    return s.items == 2 ? as(two, single) : s.items == 4 ? as(four, single) : as(eight, single);
   }
   return ugk_set_error("ugk_bucket_sort: a single tile");
 }

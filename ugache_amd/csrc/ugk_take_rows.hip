@@ -311,7 +311,7 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
   Clearing clearing(out, by_row ? 0 : num_rows * dim * elem_size(elem));
   Digits d{num_rows, 0, (1u << p.digit) - 1u, 1u << p.digit, p.digit};
   int at = 0;
-  const SortShape shape = sort_shape(n);
+  const SortShape shape = sort_shape(n, d.buckets);
   if (shape.reach == kSingle) {
     Clear clear;
     const uint32_t blocks = clearing.take(clear, 1, 1);
@@ -320,6 +320,7 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
                          (uint32_t)n, p.passes, d, clear, key[0], entry[0]);
     };
     if (shape.items == 2) one(std::integral_constant<int, 2>());
+    else if (shape.items == 4) one(std::integral_constant<int, 4>());
     else one(std::integral_constant<int, 8>());
     UGK_HIP(hipGetLastError());
   } else {
