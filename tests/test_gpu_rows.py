@@ -87,6 +87,15 @@ def test_sort(tokens, top, experts, masked):
     check_order(co.coll_torch_expert_sort(ids, experts), ids, experts)
 
 
+@pytest.mark.parametrize("tokens,top,experts", [
+    (1024, 1, 7), (1025, 1, 7), (2048, 1, 1024), (2049, 1, 64), (4095, 1, 64), (4096, 1, 2), (4097, 1, 64), (32_768, 1, 640), (32_769, 1, 1),
+    (32_769, 1, 1024), (150_001, 2, 1023), (70_000, 8, 1000), (700_000, 3, 40), (110_001, 10, 513)])
+def test_sort_where_its_shape_changes(tokens, top, experts):
+    g = gen(tokens)
+    ids = (torch.rand(tokens, top, device="cuda", generator=g) ** 2 * (experts + 1)).long() - 1  # skewed, some nowhere
+    check_order(co.coll_torch_expert_sort(ids, experts), ids, experts)
+
+
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("tokens", [40, 6000])
 def test_sort_ids_out_of_range_go_nowhere(dtype, tokens):
@@ -317,6 +326,33 @@ def test_take_rows_and_their_gradient(n, rows, dim, dtype):
     assert torch.equal(got, co.coll_torch_take_rows_grad(grad, index, rows))  # no two runs differ
 
 
+@pytest.mark.parametrize("n,rows,dim", [
+    (1024, 900, 5), (1024, 1025, 5), (1025, 5000, 3), (2048, 2048, 9), (2049, 70_001, 7), (4096, 31, 11), (4096, 100_000, 5), (4097, 4098, 5),
+    (32_768, 32_768, 3), (32_769, 32_768, 5), (32_769, 200_000, 3), (33_000, 33_001, 130), (20_000, 20_000, 257), (140_000, 1000, 33),
+    (140_000, 300_001, 7), (400_000, 2_000_000, 1), (700_000, 5, 12), (1_200_000, 1_100_000, 2)])
+@pytest.mark.parametrize("spread", [1, 4])
+def test_row_gradients_where_the_way_changes(n, rows, dim, spread):
+    g = gen(n + rows + spread)
+    index = (torch.rand(n, device="cuda", generator=g) ** spread * (rows + 2)).long() - 1  # -1 and rows among them
+    grad = randn(g, n, dim, dtype=torch.float16 if n % 2 else torch.float32)
+    got = co.coll_torch_take_rows_grad(grad, index, rows)
+    total, terms, count = plain_row_sums(grad, index, rows)
+    close(got, total, terms, count)
+    assert torch.equal(got, co.coll_torch_take_rows_grad(grad, index.int(), rows))
+
+
+@pytest.mark.parametrize("n", [50, 5000, 60_000])
+@pytest.mark.parametrize("rows", [40, 100_000])
+def test_row_gradients_in_runs_of_every_length(n, rows):
+    """rows named 0, 1, 2, ... times, so that runs of equal indices begin and end everywhere in the pieces they are summed in"""
+    times = torch.arange(n)
+    index = torch.repeat_interleave(torch.arange(n), times % 101)[:n] % rows
+    index = index[torch.randperm(n, generator=torch.Generator().manual_seed(n))].cuda()
+    grad = whole(gen(n), n, 20)
+    want = torch.zeros(rows, 20, dtype=torch.float64, device="cuda").index_add_(0, index, grad.double())
+    assert torch.equal(co.coll_torch_take_rows_grad(grad, index, rows).double(), want)
+
+
 def test_take_rows_moves_bits():
     bits = torch.randint(-2 ** 31, 2 ** 31 - 1, (50, 30), device="cuda", generator=gen(1), dtype=torch.int64).to(torch.int32)
     index = torch.randint(0, 50, (7, 11), device="cuda", generator=gen(2))
@@ -509,6 +545,19 @@ def test_norm_that_is_not_finite():
     grads[0][3] = float("nan")
     assert torch.isnan(co.coll_torch_clip_grad_norm(grads, 1.0, out=out))
     assert all(bool(torch.isnan(t).all()) for t in out)
+
+
+def test_clipping_counts_as_a_change():
+    """what autograd has saved of a tensor that is scaled in place, or written to, is stale"""
+    x, to = torch.ones(8, device="cuda", requires_grad=True), torch.zeros(8, device="cuda")
+    y = x * 2
+    loss = (y * y).sum()
+    co.coll_torch_clip_grad_norm([y.detach()], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    before = to._version
+    co.coll_torch_clip_grad_norm([x.detach()], 1.0, out=[to])
+    assert to._version > before
 
 
 def test_norm_of_other_layouts():

@@ -18,14 +18,8 @@ P = 4096  # a pointer nobody follows
 WS = 1 << 40
 
 
-class Tensor(ctypes.Structure):
-    """ugk_tensor_t"""
-    _fields_ = [("data", ctypes.c_void_p), ("out", ctypes.c_void_p), ("count", ctypes.c_uint64), ("elem", ctypes.c_int32),
-                ("reserved", ctypes.c_int32)]
-
-
 def tensors(*entries):
-    return (Tensor * len(entries))(*[Tensor(*e, 0) for e in entries])
+    return (hip.Tensor * len(entries))(*[hip.Tensor(*e, 0) for e in entries])
 
 
 @pytest.mark.parametrize("name,args,message", [
@@ -58,6 +52,11 @@ def tensors(*entries):
     ("ugk_take_rows_grad_i32", (P, 8, P, 5, 10, 64, 4, P, P, WS, None), "stride of 8"),
     ("ugk_take_rows_grad_i32", (P, 64, P, 5, 10, 64, 4, P, P, 16, None), "workspace of 16 bytes"),
     ("ugk_take_rows_grad_i32", (P, 64, P, 5, 10, 64, 4, None, P, WS, None), "null pointer"),
+    ("ugk_take_rows_grad_i32", (P, 4096, P, 1 << 26, 1 << 20, 4096, 4, P, P, WS, None), "more than one launch takes"),
+    ("ugk_take_rows_i32", (P, 10, 4096, P, 1 << 26, 4096, 4, P, None), "more than one launch takes"),
+    ("ugk_expert_dispatch", (P, 4096, P, P, 1 << 26, 2, 4096, 4, P, None), "more than one launch takes"),
+    ("ugk_expert_combine", (P, 1 << 27, 4096, P, 1 << 26, 2, P, 4, 4096, 4, P, None), "more than one launch takes"),
+    ("ugk_expert_combine_grad", (P, 4096, P, 4096, P, P, 1 << 26, 2, P, 4, 4096, 4, P, P, None), "more than one launch takes"),
     ("ugk_grad_norm", (tensors((P, None, 8, 3)), 1, P, WS, P, None), "element code 3 of tensor 0"),
     ("ugk_grad_norm", (tensors((P, None, 8, 4), (None, None, 8, 4)), 2, P, WS, P, None), "null data of tensor 1"),
     ("ugk_grad_norm", (tensors((P, None, 8, 4)), 1, P, 8, P, None), "workspace of 8 bytes"),

@@ -142,14 +142,12 @@ def build_native_rows(verbose=False):
 
 
 def build_all(verbose=False):
-    # the module over torch's headers takes as long as the longest kernel source: side by side with the rest
-    from concurrent.futures import ThreadPoolExecutor
+    import importlib.util
     build_hip(verbose)
-    with ThreadPoolExecutor(max_workers=1) as pool:
-        rows = pool.submit(build_native_rows, verbose)
-        build_host(verbose)
-        build_native_c_lib(verbose)
-        rows.result()
+    build_host(verbose)
+    build_native_c_lib(verbose)
+    if importlib.util.find_spec("torch") is not None:  # the C libraries are of use without it
+        build_native_rows(verbose)
 
 
 if __name__ == "__main__":

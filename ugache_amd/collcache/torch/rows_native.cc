@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <pybind11/pybind11.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -260,7 +261,7 @@ py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h)
       throw py::value_error(std::to_string(outs.size()) + " outputs for " + std::to_string(grads.size()) + " gradients");
   }
   std::vector<ugk_tensor_t> listed;
-  std::vector<Tensor> copies;
+  std::vector<Tensor> copies, changed;
   std::vector<const void *> written;
   listed.reserve(grads.size());
   Tensor first;
@@ -281,6 +282,9 @@ py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h)
       if (o.scalar_type() != g.scalar_type() || o.sizes() != g.sizes() || !o.is_contiguous())
         throw py::value_error("an output must be contiguous and of its gradient's shape, type and GPU");
       to = o.data_ptr();
+      changed.push_back(o);
+    } else if (clip) {
+      changed.push_back(g);
     }
     listed.push_back(ugk_tensor_t{g.data_ptr(), to, (uint64_t)g.numel(), ElemOf(g), 0});
     if (clip && g.numel()) written.push_back(to);
@@ -290,6 +294,7 @@ py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h)
   if (std::adjacent_find(written.begin(), written.end()) != written.end())
     throw py::value_error("two gradients are written to the same place");
   const On on(first);
+  for (const Tensor &t : changed) t.unsafeGetTensorImpl()->bump_version();  // what autograd has saved of them is stale
   const size_t nbytes = ugk_grad_norm_workspace_bytes(listed.data(), listed.size());
   Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
   const Tensor scratch = Scratch(nbytes, first);
@@ -298,18 +303,33 @@ py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h)
   return Wrap(std::move(norm));
 }
 
+// torch's exceptions reach Python as torch's own (out of memory among them)
+template <typename R, typename... A>
+auto Guarded(R (*f)(A...)) {
+  return [f](A... args) -> R {
+    HANDLE_TH_ERRORS
+    return f(args...);
+    END_HANDLE_TH_ERRORS_PYBIND
+  };
+}
+
+py::object CombineRows(py::handle rows, py::handle slot, py::handle offsets, py::handle weights) {
+  return Combine("rows", rows, slot, offsets, weights);
+}
+py::object DispatchGrad(py::handle rows, py::handle slot, py::handle offsets) { return Combine("grad_rows", rows, slot, offsets, py::none()); }
+
 }  // namespace
 
 PYBIND11_MODULE(rows_native, m) {
   m.doc() = "the calls of collcache.torch.rows, compiled";
   g_raw_stream = py::object(py::module_::import("torch._C").attr("_cuda_getCurrentRawStream")).release().ptr();
   g_launch_error = py::object(py::module_::import("builtins").attr("RuntimeError")).release().ptr();
-  m.def("expert_sort", &ExpertSort);
-  m.def("dispatch", &Dispatch);
-  m.def("combine", [](py::handle r, py::handle s, py::handle o, py::handle w) { return Combine("rows", r, s, o, w); });
-  m.def("dispatch_grad", [](py::handle r, py::handle s, py::handle o) { return Combine("grad_rows", r, s, o, py::none()); });
-  m.def("combine_grad", &CombineGrad);
-  m.def("take_rows", &TakeRows);
-  m.def("take_rows_grad", &TakeRowsGrad);
-  m.def("grad_norm", &GradNorm);
+  m.def("expert_sort", Guarded(&ExpertSort));
+  m.def("dispatch", Guarded(&Dispatch));
+  m.def("dispatch_grad", Guarded(&DispatchGrad));
+  m.def("combine", Guarded(&CombineRows));
+  m.def("combine_grad", Guarded(&CombineGrad));
+  m.def("take_rows", Guarded(&TakeRows));
+  m.def("take_rows_grad", Guarded(&TakeRowsGrad));
+  m.def("grad_norm", Guarded(&GradNorm));
 }

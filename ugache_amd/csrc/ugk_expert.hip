@@ -220,7 +220,7 @@ int ugk_expert_dispatch(const void *x_dev, size_t x_stride, const int32_t *slot_
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(tokens, s);
-    UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_expert_dispatch: %zu tokens of %zu elements are more than one launch takes", tokens, dim);
+    UGK_REQUIRE(blocks <= kMaxBlocks, "ugk_expert_dispatch: %zu tokens of %zu elements are more than one launch takes", tokens, dim);
     hipLaunchKernelGGL((dispatch_kernel<T, V, decltype(stream_out)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)x_dev, x_stride,
                        slot_dev, live_dev, tokens, top, (uint32_t)dim, s, (T *)rows_dev);
     UGK_HIP(hipGetLastError());
@@ -240,7 +240,7 @@ int ugk_expert_combine(const void *rows_dev, size_t n_rows, size_t row_stride, c
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(tokens, s);
-    UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_expert_combine: %zu tokens of %zu elements are more than one launch takes", tokens, dim);
+    UGK_REQUIRE(blocks <= kMaxBlocks, "ugk_expert_combine: %zu tokens of %zu elements are more than one launch takes", tokens, dim);
     hipLaunchKernelGGL((combine_kernel<T, V, decltype(stream_rows)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)rows_dev, row_stride,
                        (uint32_t)n_rows, slot_dev, tokens, top, weights_dev, weight_elem, (uint32_t)dim, s, (T *)out_dev);
     UGK_HIP(hipGetLastError());
@@ -274,8 +274,9 @@ int ugk_expert_combine_grad(const void *grad_out_dev, size_t grad_stride, const 
       UGK_HIP(hipGetLastError());
       return 0;
     };
-    const size_t per = kBlock / lanes;
-    return wide ? launch(std::true_type(), tokens, kBlock) : launch(std::false_type(), (tokens + per - 1) / per, lanes);
+    const size_t per = kBlock / lanes, blocks = wide ? tokens : (tokens + per - 1) / per;
+    UGK_REQUIRE(blocks <= kMaxBlocks, "ugk_expert_combine_grad: %zu tokens are more than one launch takes", tokens);
+    return wide ? launch(std::true_type(), blocks, kBlock) : launch(std::false_type(), blocks, lanes);
   });
 }
 

@@ -221,7 +221,7 @@ int for_lists(const ugk_tensor_t *tensors, size_t n, bool backwards, F launch) {
     for (uint64_t j = 0; j < parts; ++j) {
       const uint64_t from = (backwards ? parts - 1 - j : j) * kPartElems, count = std::min(kPartElems, t.count - from);
       const uint32_t more = pieces_in(count, t.elem);
-      if (list.n > 0 && (list.n == (uint32_t)kListed || (uint64_t)list.pieces + more >= ((uint64_t)1 << 31))) {
+      if (list.n > 0 && (list.n == (uint32_t)kListed || (uint64_t)list.pieces + more > kMaxBlocks)) {
         if (int rc = launch(list, before)) return rc;
         before += list.pieces;
         list.n = list.pieces = 0;

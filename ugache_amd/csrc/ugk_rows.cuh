@@ -126,6 +126,14 @@ static inline int for_moved_rows(int elem, size_t dim, size_t out_rows, F f) {
   return dim >= 8 ? stored(uint16_t(), std::integral_constant<int, 8>()) : stored(uint16_t(), std::integral_constant<int, 1>());
 }
 
+// the work-items of a launch are counted in 32 bits
+constexpr size_t kMaxBlocks = ((size_t)1 << 32) / kBlock - 1;
+
+static inline size_t chunks_of(int elem, size_t dim) {  // of a row
+  const size_t vec = elem == 4 ? 4 : 8;
+  return dim >= vec ? (dim + vec - 1) / vec : dim;
+}
+
 static inline bool elem_ok(int elem) { return elem == 4 || elem == 2 || elem == UGK_ELEM_BF16; }
 static inline size_t elem_size(int elem) { return elem == 4 ? 4 : 2; }
 

@@ -187,17 +187,18 @@ __global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ g
 // The parts of a row added up: a workgroup per run in which such a row begins and per `lanes` chunks of it.  kBlock / lanes
 // groups of lanes add consecutive parts each, then the groups' sums are added in their order.
 template <typename T, int VEC, bool BY_ROW>
-__global__ __launch_bounds__(kBlock) void row_join_kernel(Sorted s, uint32_t dim, uint32_t chunks, uint32_t lanes,
+__global__ __launch_bounds__(kBlock) void row_join_kernel(Sorted s, uint32_t dim, uint32_t chunks, uint32_t lanes, uint32_t columns,
                                                           const float *__restrict__ parts, T *__restrict__ out) {
   __shared__ float held[kBlock * VEC];
+  const uint32_t p0 = blockIdx.x / columns, column = blockIdx.x - p0 * columns;
   uint32_t r, from, to;
-  if (!long_row_from<BY_ROW>(s, blockIdx.x, r, from, to)) return;
+  if (!long_row_from<BY_ROW>(s, p0, r, from, to)) return;
   if constexpr (BY_ROW) to = s.begin[r + 1];
   else to = wave_first_of(s.keys, to, s.n, r + 1);
   const uint32_t group = threadIdx.x / lanes, groups = kBlock / lanes;  // lanes: a power of two
-  const uint32_t c = blockIdx.y * lanes + threadIdx.x % lanes;
+  const uint32_t c = column * lanes + threadIdx.x % lanes;
   const uint32_t at = min(c * VEC, dim - VEC);
-  const uint32_t p0 = blockIdx.x, pieces = (to - 1) / s.piece - p0 + 1;
+  const uint32_t pieces = (to - 1) / s.piece - p0 + 1;
   const uint32_t per = (pieces + groups - 1) / groups;
   float sum[VEC] = {};
   if (c < chunks) {
@@ -248,7 +249,7 @@ int take_rows(const void *table, uint64_t num_rows, size_t stride, const I *inde
     constexpr int V = decltype(vec)::value;
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(n, s);
-    UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_take_rows: %zu rows of %zu elements are more than one launch takes", n, dim);
+    UGK_REQUIRE(blocks <= kMaxBlocks, "ugk_take_rows: %zu rows of %zu elements are more than one launch takes", n, dim);
     hipLaunchKernelGGL((take_rows_kernel<T, V, decltype(stream_out)::value, I>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)table, num_rows,
                        stride, index, n, (uint32_t)dim, s, (T *)out);
     UGK_HIP(hipGetLastError());
@@ -290,6 +291,9 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
   UGK_REQUIRE(n < ((size_t)1 << 31) && num_rows < ((uint64_t)1 << 31), "ugk_take_rows_grad: %zu entries of %zu rows, both have 31 bits", n,
               (size_t)num_rows);
   UGK_REQUIRE(stride >= dim || n <= 1, "ugk_take_rows_grad: rows of %zu elements overlap at a stride of %zu", dim, stride);
+  // a workgroup's 256 chunks, of the rows, of the entries and of the parts
+  UGK_REQUIRE((num_rows + 2 * n) * chunks_of(elem, dim) / kBlock + 2 < kMaxBlocks,
+              "ugk_take_rows_grad: %zu rows and %zu entries of %zu elements are more than one launch takes", (size_t)num_rows, n, dim);
   if (num_rows == 0) return 0;
   UGK_REQUIRE(out && (n == 0 || (grad && index)), "ugk_take_rows_grad: null pointer");
   const size_t need = ugk_take_rows_grad_workspace_bytes(n, num_rows, dim);
@@ -343,16 +347,16 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
     const Sorted sorted{key[at], begin, (uint32_t)n, (uint32_t)num_rows, piece};
     const size_t pieces = n > piece ? pieces_of(n, dim) : 0;  // in fewer entries no row has more than a piece
     const size_t row_blocks = split_blocks(by_row ? num_rows : n, s), blocks = row_blocks + split_blocks(pieces, s);
-    UGK_REQUIRE(blocks < ((size_t)1 << 31), "ugk_take_rows_grad: %zu rows of %zu elements are more than one launch takes", (size_t)num_rows, dim);
     uint32_t lanes = 1;
     while (lanes < s.chunks && lanes < 32) lanes *= 2;
+    const uint32_t columns = (s.chunks + lanes - 1) / lanes;
     const auto launch = [&](auto rowwise, auto stored) {
       constexpr bool R = decltype(rowwise)::value;
       hipLaunchKernelGGL((row_sum_kernel<T, V, R, decltype(stored)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),
                          (const T *)grad, stride, entry[at], sorted, (uint32_t)dim, s, (uint32_t)row_blocks, (T *)out, parts);
       if (pieces > 0)
-        hipLaunchKernelGGL((row_join_kernel<T, V, R>), dim3((unsigned)pieces, (s.chunks + lanes - 1) / lanes), dim3(kBlock), 0, as_stream(stream),
-                           sorted, (uint32_t)dim, s.chunks, lanes, parts, (T *)out);
+        hipLaunchKernelGGL((row_join_kernel<T, V, R>), dim3((unsigned)pieces * columns), dim3(kBlock), 0, as_stream(stream), sorted,
+                           (uint32_t)dim, s.chunks, lanes, columns, parts, (T *)out);
     };
     if (by_row) launch(std::true_type(), stream_out);
     else launch(std::false_type(), std::false_type());

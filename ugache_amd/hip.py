@@ -57,6 +57,11 @@ class Handed(C.Structure):
     _fields_ = [("stamps", C.c_void_p), ("used_bits", C.c_void_p), ("nslots", C.c_uint64)]
 
 
+class Tensor(C.Structure):
+    """ugk_tensor_t"""
+    _fields_ = [("data", C.c_void_p), ("out", C.c_void_p), ("count", C.c_uint64), ("elem", C.c_int32), ("reserved", C.c_int32)]
+
+
 class DeviceInfo(C.Structure):
     """ugk_device_info_t"""
     _fields_ = [("name", C.c_char * 256), ("arch", C.c_char * 64), ("compute_units", C.c_int32),
