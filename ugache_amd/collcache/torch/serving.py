@@ -233,10 +233,10 @@ class SparseLookupLayer(torch.nn.Module):
         if self.unique_in_library:  # unique + lookup in one call, the unique by the library's GPU hash set
             self.lookup.check(ids)
             emb_unique, idx = _adapter.coll_torch_lookup_unique(0, ids)
-            embeddings = emb_unique.index_select(0, idx.long())
+            embeddings = _adapter.coll_torch_take_rows(emb_unique, idx)
         else:
             ids, idx = torch.unique(ids, return_inverse=True)
-            embeddings = self.lookup(ids).index_select(0, idx)
+            embeddings = _adapter.coll_torch_take_rows(self.lookup(ids), idx)
         original_dtype = embeddings.dtype
         if embeddings.dtype in (torch.float16, torch.bfloat16):
             embeddings = embeddings.float()  # low-precision rows are combined in fp32

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kBlock) void combine_kernel(const T *__restrict__ r
   if (t >= tokens) return;
   const uint32_t at = min(c * VEC, dim - VEC);
   float sum[VEC] = {};
-  constexpr uint32_t U = 8;  // rows on their way
+  constexpr uint32_t U = 4;  // rows on their way (8: the same for eight experts a token, 65 us against 58 for two)
   for (uint32_t k0 = 0; k0 < top; k0 += U) {
     const size_t i = t * top + k0;
     const uint32_t last = min(U, top - k0) - 1;
