@@ -221,8 +221,8 @@ int ugk_expert_dispatch(const void *x_dev, size_t x_stride, const int32_t *slot_
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(tokens, s);
     UGK_REQUIRE(blocks <= kMaxBlocks, "ugk_expert_dispatch: %zu tokens of %zu elements are more than one launch takes", tokens, dim);
-    hipLaunchKernelGGL((dispatch_kernel<T, V, decltype(stream_out)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)x_dev, x_stride,
-                       slot_dev, live_dev, tokens, top, (uint32_t)dim, s, (T *)rows_dev);
+    hipLaunchKernelGGL((dispatch_kernel<T, V, decltype(stream_out)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),
+                       (const T *)x_dev, x_stride, slot_dev, live_dev, tokens, top, (uint32_t)dim, s, (T *)rows_dev);
     UGK_HIP(hipGetLastError());
     return 0;
   });
@@ -241,8 +241,8 @@ int ugk_expert_combine(const void *rows_dev, size_t n_rows, size_t row_stride, c
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(tokens, s);
     UGK_REQUIRE(blocks <= kMaxBlocks, "ugk_expert_combine: %zu tokens of %zu elements are more than one launch takes", tokens, dim);
-    hipLaunchKernelGGL((combine_kernel<T, V, decltype(stream_rows)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)rows_dev, row_stride,
-                       (uint32_t)n_rows, slot_dev, tokens, top, weights_dev, weight_elem, (uint32_t)dim, s, (T *)out_dev);
+    hipLaunchKernelGGL((combine_kernel<T, V, decltype(stream_rows)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),
+                       (const T *)rows_dev, row_stride, (uint32_t)n_rows, slot_dev, tokens, top, weights_dev, weight_elem, (uint32_t)dim, s, (T *)out_dev);
     UGK_HIP(hipGetLastError());
     return 0;
   });
@@ -252,9 +252,11 @@ int ugk_expert_combine_grad(const void *grad_out_dev, size_t grad_stride, const 
                             const int32_t *live_dev, size_t tokens, uint32_t top, const void *weights_dev, int weight_elem, size_t dim,
                             int elem, void *grad_rows_dev, void *grad_weights_dev, void *stream) {
   if (int rc = check_rows("ugk_expert_combine_grad", tokens, top, dim, elem, grad_stride)) return rc;
-  UGK_REQUIRE(row_stride >= dim || tokens * top <= 1 || !grad_weights_dev, "ugk_expert_combine_grad: rows of %zu elements overlap at a stride of %zu",
+  UGK_REQUIRE(row_stride >= dim || tokens * top <= 1 || !grad_weights_dev,
+              "ugk_expert_combine_grad: rows of %zu elements overlap at a stride of %zu",
               dim, row_stride);
-  UGK_REQUIRE((!weights_dev && !grad_weights_dev) || elem_ok(weight_elem), "ugk_expert_combine_grad: element code %d of the weights", weight_elem);
+  UGK_REQUIRE((!weights_dev && !grad_weights_dev) || elem_ok(weight_elem),
+              "ugk_expert_combine_grad: element code %d of the weights", weight_elem);
   if (tokens == 0) return 0;
   UGK_REQUIRE(grad_out_dev && slot_dev && live_dev && grad_rows_dev && (rows_dev || !grad_weights_dev), "ugk_expert_combine_grad: null pointer");
   return for_rows_streamed(elem, dim, tokens * top, [&](auto type, auto vec, auto stream_rows) -> int {

@@ -35,7 +35,12 @@ __device__ __forceinline__ uint32_t first_of(const uint32_t *keys, uint32_t lo, 
   }
   return lo;
 }
-// the same for a wavefront that searches for one row: 64 keys a step
+// the first position behind `at` where another row's keys begin; `at` is row r's or the one behind its last
+__device__ __forceinline__ uint32_t end_of(const uint32_t *keys, uint32_t at, uint32_t n, uint32_t r, uint32_t step) {
+  while (step < n - at && keys[at + step] == r) at += step, step *= 2;
+  return first_of(keys, at, min(at + min(step, n - at) + 1, n), r + 1);
+}
+// the same as first_of for a wavefront that searches for one row: 64 keys a step
 __device__ __forceinline__ uint32_t wave_first_of(const uint32_t *keys, uint32_t lo, uint32_t hi, uint32_t r) {
   while (hi > lo) {
     const uint32_t step = (hi - lo + kWave - 1) / kWave, at = lo + lane_id() * step;
@@ -98,23 +103,29 @@ struct Sorted {
   uint32_t n, rows, piece;
 };
 
+// (Keys that a decision needs are loaded together, whether or not the first of them settles it: they were written by another
+// XCD and are a microsecond away each.)
+
 // whether a row that is summed in pieces begins in a run; the row, its first position, and where the run's entries end
 template <bool BY_ROW>
 __device__ __forceinline__ bool long_row_from(const Sorted &s, uint32_t run, uint32_t &row, uint32_t &first, uint32_t &to) {
   const uint32_t from = run * s.piece;
+  to = min(from + s.piece, s.n);
+  row = s.keys[to - 1];
   if constexpr (BY_ROW) {
     const uint32_t live = s.begin[s.rows];
-    if (from >= live) return false;
-    to = min(from + s.piece, live);
-    row = s.keys[to - 1];
+    if (row >= s.rows) {  // entries without a row come last
+      if (from >= live) return false;
+      to = live;
+      row = s.keys[to - 1];
+    }
     first = s.begin[row];
     return first >= from && s.begin[row + 1] - first > s.piece;
   } else {
-    to = min(from + s.piece, s.n);
-    row = s.keys[to - 1];
+    const uint32_t behind = s.keys[min(to, s.n - 1)], head = s.keys[from], before = s.keys[max(from, 1u) - 1];
     // it goes on behind the run, and did not begin before it
-    if (row >= s.rows || to == s.n || s.keys[to] != row || (from > 0 && s.keys[from - 1] == row)) return false;
-    first = first_of(s.keys, from, to, row);
+    if (row >= s.rows || to == s.n || behind != row || (from > 0 && before == row)) return false;
+    first = head == row ? from : first_of(s.keys, from + 1, to, row);
     return first + s.piece < s.n && s.keys[first + s.piece] == row;
   }
 }
@@ -124,16 +135,17 @@ __device__ __forceinline__ bool long_row_into(const Sorted &s, uint32_t run, uin
   const uint32_t from = run * s.piece, to = min(from + s.piece, s.n);
   if (from >= s.n || from == 0) return false;
   const uint32_t row = s.keys[from];
-  if (row >= s.rows) return false;
   if constexpr (BY_ROW) {
+    if (row >= s.rows) return false;
     const uint32_t first = s.begin[row], last = s.begin[row + 1];
     end = min(to, last);
     return first < from && last - first > s.piece;
   } else {
-    if (s.keys[from - 1] != row) return false;
-    const uint32_t first = s.keys[from - s.piece] == row ? from - s.piece : first_of(s.keys, from - s.piece, from, row);
+    const uint32_t before = s.keys[from - 1], back = s.keys[from - s.piece], tail = s.keys[to - 1];
+    if (row >= s.rows || before != row) return false;
+    const uint32_t first = back == row ? from - s.piece : first_of(s.keys, from - s.piece + 1, from, row);
     if (first + s.piece >= s.n || s.keys[first + s.piece] != row) return false;
-    end = s.keys[to - 1] == row ? to : first_of(s.keys, from, to, row + 1);
+    end = tail == row ? to : first_of(s.keys, from + 1, to, row + 1);
     return true;
   }
 }
@@ -159,11 +171,11 @@ __global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ g
     } else {
       if (i >= s.n) return;
       from = (uint32_t)i;
-      const uint32_t r = s.keys[from];
-      if (r >= s.rows || (from > 0 && s.keys[from - 1] == r)) return;
       to = min(from + s.piece, s.n);
-      if (to < s.n && s.keys[to] == r) return;
-      to = from + 1 < s.n && s.keys[from + 1] == r ? first_of(s.keys, from + 2, to, r + 1) : from + 1;
+      const uint32_t r = s.keys[from], before = s.keys[max(from, 1u) - 1], next = s.keys[min(from + 1, s.n - 1)],
+                     behind = s.keys[min(to, s.n - 1)];
+      if (r >= s.rows || (from > 0 && before == r) || (to < s.n && behind == r)) return;
+      to = from + 1 < s.n && next == r ? first_of(s.keys, from + 2, to, r + 1) : from + 1;
       i = r;
     }
     add_entries<T, VEC>(grad, stride, entries, from, to, at, sum);
@@ -184,47 +196,74 @@ __global__ __launch_bounds__(kBlock) void row_sum_kernel(const T *__restrict__ g
   }
 }
 
-// The parts of a row added up: a workgroup per run in which such a row begins and per `lanes` chunks of it.  kBlock / lanes
-// groups of lanes add consecutive parts each, then the groups' sums are added in their order.
+// sum += the parts from .. to of a row whose first is in run p0
+template <int VEC>
+__device__ __forceinline__ void add_parts(const float *parts, uint32_t dim, uint32_t p0, uint32_t from, uint32_t to, uint32_t at,
+                                          float (&sum)[VEC]) {
+  constexpr uint32_t U = 8;  // parts on their way
+  for (uint32_t p = from; p < to; p += U) {
+    float v[U][VEC];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t q = min(p + u, to - 1);
+      load_chunk<float, VEC>(parts + (2 * (size_t)(p0 + q) + (q == 0 ? 1 : 0)) * dim + at, v[u]);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] += p + u < to ? v[u][e] : 0.f;
+  }
+}
+
+// The parts of a row added up, for `lanes` chunks of it.  A group of `lanes` lanes looks after a run: if a row that is summed
+// in pieces begins there it adds the row's parts; those of a row of many parts the workgroup's kBlock / lanes groups add
+// together, consecutive ones each, and the groups' sums are added in their order.  (us of the gradient, many from 8 / 16 / 32 /
+// 64 on: 16,384 entries over 50,000 rows, 8 groups 46.0 / 46.0 / 47.2 / 51.9; 202,156 over 3,277 rows of 16 bytes, 256 groups
+// 150 / 105 / 80 / 72.)
 template <typename T, int VEC, bool BY_ROW>
-__global__ __launch_bounds__(kBlock) void row_join_kernel(Sorted s, uint32_t dim, uint32_t chunks, uint32_t lanes, uint32_t columns,
+__global__ __launch_bounds__(kBlock) void row_join_kernel(Sorted s, uint32_t runs, uint32_t dim, uint32_t chunks, uint32_t lanes, uint32_t columns,
                                                           const float *__restrict__ parts, T *__restrict__ out) {
   __shared__ float held[kBlock * VEC];
-  const uint32_t p0 = blockIdx.x / columns, column = blockIdx.x - p0 * columns;
-  uint32_t r, from, to;
-  if (!long_row_from<BY_ROW>(s, p0, r, from, to)) return;
-  if constexpr (BY_ROW) to = s.begin[r + 1];
-  else to = wave_first_of(s.keys, to, s.n, r + 1);
+  __shared__ uint32_t many[kBlock][3], n_many;  // rows of many parts: the row, its first run, its parts
+  if (threadIdx.x == 0) n_many = 0;
+  __syncthreads();
   const uint32_t group = threadIdx.x / lanes, groups = kBlock / lanes;  // lanes: a power of two
+  const uint32_t run0 = blockIdx.x / columns * groups, column = blockIdx.x % columns;
   const uint32_t c = column * lanes + threadIdx.x % lanes;
   const uint32_t at = min(c * VEC, dim - VEC);
-  const uint32_t pieces = (to - 1) / s.piece - p0 + 1;
-  const uint32_t per = (pieces + groups - 1) / groups;
-  float sum[VEC] = {};
-  if (c < chunks) {
-    constexpr uint32_t U = 8;  // parts on their way
-    const uint32_t end = min((group + 1) * per, pieces);
-    for (uint32_t p = group * per; p < end; p += U) {
-      float v[U][VEC];
-#pragma unroll
-      for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t q = min(p + u, end - 1);
-        load_chunk<float, VEC>(parts + (2 * (size_t)(p0 + q) + (q == 0 ? 1 : 0)) * dim + at, v[u]);
-      }
-#pragma unroll
-      for (uint32_t u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum[e] += p + u < end ? v[u][e] : 0.f;
-    }
+  const uint32_t run = run0 + group, few = max(16u, groups / 4);
+  uint32_t r = 0, from = 0, to = 0, pieces = 0;
+  if (run < runs && long_row_from<BY_ROW>(s, run, r, from, to)) {
+    if constexpr (BY_ROW) to = s.begin[r + 1];
+    else to = end_of(s.keys, to, s.n, r, s.piece);
+    pieces = (to - 1) / s.piece - run + 1;
   }
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) held[e * kBlock + threadIdx.x] = sum[e];
+  if (threadIdx.x % lanes == 0 && pieces > few) {
+    const uint32_t g = atomicAdd(&n_many, 1u);  // rows are added up one by one: in whatever order
+    many[g][0] = r, many[g][1] = run, many[g][2] = pieces;
+  }
+  if (pieces > 0 && pieces <= few && c < chunks) {
+    float sum[VEC] = {};
+    add_parts<VEC>(parts, dim, run, 0, pieces, at, sum);
+    store_chunk<T, VEC>(out + (size_t)r * dim + at, sum);
+  }
   __syncthreads();
-  if (group != 0 || c >= chunks) return;
-  for (uint32_t g = 1; g < groups; ++g)
+  for (uint32_t g = 0; g < n_many; ++g) {
+    pieces = many[g][2];
+    const uint32_t per = (pieces + groups - 1) / groups;
+    float sum[VEC] = {};
+    if (c < chunks) add_parts<VEC>(parts, dim, many[g][1], min(group * per, pieces), min((group + 1) * per, pieces), at, sum);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) sum[e] += held[e * kBlock + g * lanes + threadIdx.x];
-  store_chunk<T, VEC>(out + (size_t)r * dim + at, sum);
+    for (int e = 0; e < VEC; ++e) held[e * kBlock + threadIdx.x] = sum[e];
+    __syncthreads();
+    if (group == 0 && c < chunks) {
+      for (uint32_t h = 1; h < groups; ++h)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] += held[e * kBlock + h * lanes + threadIdx.x];
+      store_chunk<T, VEC>(out + (size_t)many[g][0] * dim + at, sum);
+    }
+    __syncthreads();
+  }
 }
 
 // more of the output than the sort's launches clear on their side
@@ -250,8 +289,8 @@ int take_rows(const void *table, uint64_t num_rows, size_t stride, const I *inde
     const Split s = split_of(dim, V);
     const size_t blocks = split_blocks(n, s);
     UGK_REQUIRE(blocks <= kMaxBlocks, "ugk_take_rows: %zu rows of %zu elements are more than one launch takes", n, dim);
-    hipLaunchKernelGGL((take_rows_kernel<T, V, decltype(stream_out)::value, I>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream), (const T *)table, num_rows,
-                       stride, index, n, (uint32_t)dim, s, (T *)out);
+    hipLaunchKernelGGL((take_rows_kernel<T, V, decltype(stream_out)::value, I>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),
+                       (const T *)table, num_rows, stride, index, n, (uint32_t)dim, s, (T *)out);
     UGK_HIP(hipGetLastError());
     return 0;
   });
@@ -297,7 +336,8 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
   if (num_rows == 0) return 0;
   UGK_REQUIRE(out && (n == 0 || (grad && index)), "ugk_take_rows_grad: null pointer");
   const size_t need = ugk_take_rows_grad_workspace_bytes(n, num_rows, dim);
-  UGK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "ugk_take_rows_grad: a workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+  UGK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "ugk_take_rows_grad: a workspace of %zu bytes, %zu are needed",
+              workspace_bytes, need);
   uint32_t *begin = static_cast<uint32_t *>(workspace);
   uint32_t *key[2] = {begin + begin_words(n, num_rows, dim), begin + begin_words(n, num_rows, dim) + n}, *entry[2] = {key[1] + n, key[1] + 2 * n};
   float *parts = reinterpret_cast<float *>(entry[1] + n);
@@ -355,8 +395,8 @@ int take_rows_grad(const void *grad, size_t stride, const I *index, size_t n, ui
       hipLaunchKernelGGL((row_sum_kernel<T, V, R, decltype(stored)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),
                          (const T *)grad, stride, entry[at], sorted, (uint32_t)dim, s, (uint32_t)row_blocks, (T *)out, parts);
       if (pieces > 0)
-        hipLaunchKernelGGL((row_join_kernel<T, V, R>), dim3((unsigned)pieces * columns), dim3(kBlock), 0, as_stream(stream), sorted,
-                           (uint32_t)dim, s.chunks, lanes, columns, parts, (T *)out);
+        hipLaunchKernelGGL((row_join_kernel<T, V, R>), dim3((unsigned)((pieces + kBlock / lanes - 1) / (kBlock / lanes)) * columns),
+                           dim3(kBlock), 0, as_stream(stream), sorted, (uint32_t)pieces, (uint32_t)dim, s.chunks, lanes, columns, parts, (T *)out);
     };
     if (by_row) launch(std::true_type(), stream_out);
     else launch(std::false_type(), std::false_type());
