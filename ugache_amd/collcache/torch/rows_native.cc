@@ -235,14 +235,31 @@ py::object TakeRowsGrad(py::handle grad_h, py::handle index_h, int64_t num_rows)
   return Wrap(std::move(out));
 }
 
-std::vector<py::object> ListOf(py::handle h) {
-  std::vector<py::object> items;
-  if (THPVariable_Check(h.ptr())) {
-    items.push_back(py::reinterpret_borrow<py::object>(h));
-    return items;
+// a sequence of tensors, or one tensor, held while the call runs
+class Items {
+ public:
+  explicit Items(py::handle h) {
+    if (THPVariable_Check(h.ptr())) {
+      _one = h.ptr();
+      return;
+    }
+    _seq = py::reinterpret_steal<py::object>(PySequence_Fast(h.ptr(), "gradients must be a tensor or a sequence of tensors"));
+    if (!_seq) throw py::error_already_set();
   }
-  for (py::handle item : py::iter(h)) items.push_back(py::reinterpret_borrow<py::object>(item));
-  return items;
+  size_t size() const { return _one ? 1 : (size_t)PySequence_Fast_GET_SIZE(_seq.ptr()); }
+  PyObject *operator[](size_t i) const { return _one ? _one : PySequence_Fast_GET_ITEM(_seq.ptr(), (Py_ssize_t)i); }
+
+ private:
+  PyObject *_one = nullptr;
+  py::object _seq;
+};
+
+const Tensor &ListedTensor(const char *what, PyObject *o, int dev) {
+  const Tensor *t = THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+  if (!t || !t->is_cuda() || t->layout() != c10::kStrided || ElemOf(*t) == 0)
+    throw py::type_error(std::string(what) + " must be a GPU tensor of float32, float16, bfloat16");
+  if (dev >= 0 && t->get_device() != dev) throw py::value_error(std::string(what) + " must be on the GPU of the other tensors");
+  return *t;
 }
 
 // max_norm None: the norm alone; out None: in place
@@ -253,51 +270,52 @@ py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h)
     max_norm = max_norm_h.cast<double>();
     if (!(max_norm >= 0)) throw py::value_error("max_norm must be at least 0, got " + std::to_string(max_norm));
   }
-  const std::vector<py::object> grads = ListOf(grads_h);
-  std::vector<py::object> outs;
-  if (elsewhere) {
-    outs = ListOf(out_h);
-    if (outs.size() != grads.size())
-      throw py::value_error(std::to_string(outs.size()) + " outputs for " + std::to_string(grads.size()) + " gradients");
-  }
+  const Items grads(grads_h), outs(elsewhere ? out_h : grads_h);
+  const size_t n = grads.size();
+  if (outs.size() != n) throw py::value_error(std::to_string(outs.size()) + " outputs for " + std::to_string(n) + " gradients");
   std::vector<ugk_tensor_t> listed;
-  std::vector<Tensor> copies, changed;
+  std::vector<Tensor> copies;
   std::vector<const void *> written;
-  listed.reserve(grads.size());
-  Tensor first;
-  for (size_t i = 0; i < grads.size(); ++i) {
-    if (grads[i].is_none()) continue;
-    Tensor g = Unpack("a gradient", grads[i], kRowsKind, first.defined() ? (int)first.get_device() : -1);
-    if (!first.defined()) first = g;
+  std::vector<c10::TensorImpl *> changed;
+  listed.reserve(n);
+  written.reserve(n);
+  changed.reserve(n);
+  const Tensor *first = nullptr;
+  int dev = -1;
+  for (size_t i = 0; i < n; ++i) {
+    if (grads[i] == Py_None) continue;
+    const Tensor *g = &ListedTensor("a gradient", grads[i], dev);
+    if (!first) first = g, dev = (int)g->get_device();
     // in place and for the norm alone the order of the elements is nobody's matter, so long as they are one run of memory
-    if (!g.is_contiguous() && (elsewhere || !g.is_non_overlapping_and_dense())) {
-      if (clip && !elsewhere && g.numel())
+    if (!g->is_contiguous() && (elsewhere || !g->is_non_overlapping_and_dense())) {
+      if (clip && !elsewhere && g->numel())
         throw py::value_error("a gradient whose elements are no run of memory cannot be scaled in place");
-      g = g.contiguous();
-      copies.push_back(g);
+      copies.push_back(g->contiguous());
+      g = nullptr;
     }
-    void *to = g.data_ptr();
+    const Tensor &from = g ? *g : copies.back();
+    void *at = from.data_ptr(), *to = at;
     if (elsewhere) {
-      const Tensor o = Unpack("an output", outs[i], kRowsKind, (int)first.get_device());
-      if (o.scalar_type() != g.scalar_type() || o.sizes() != g.sizes() || !o.is_contiguous())
+      const Tensor &o = ListedTensor("an output", outs[i], dev);
+      if (o.scalar_type() != from.scalar_type() || o.sizes() != from.sizes() || !o.is_contiguous())
         throw py::value_error("an output must be contiguous and of its gradient's shape, type and GPU");
       to = o.data_ptr();
-      changed.push_back(o);
+      changed.push_back(o.unsafeGetTensorImpl());
     } else if (clip) {
-      changed.push_back(g);
+      changed.push_back(from.unsafeGetTensorImpl());
     }
-    listed.push_back(ugk_tensor_t{g.data_ptr(), to, (uint64_t)g.numel(), ElemOf(g), 0});
-    if (clip && g.numel()) written.push_back(to);
+    listed.push_back(ugk_tensor_t{at, to, (uint64_t)from.numel(), ElemOf(from), 0});
+    if (clip && from.numel()) written.push_back(to);
   }
-  if (!first.defined()) throw py::value_error("no gradients");
+  if (!first) throw py::value_error("no gradients");
   std::sort(written.begin(), written.end());
   if (std::adjacent_find(written.begin(), written.end()) != written.end())
     throw py::value_error("two gradients are written to the same place");
-  const On on(first);
-  for (const Tensor &t : changed) t.unsafeGetTensorImpl()->bump_version();  // what autograd has saved of them is stale
+  const On on(*first);
+  for (c10::TensorImpl *t : changed) t->bump_version();  // what autograd has saved of them is stale
   const size_t nbytes = ugk_grad_norm_workspace_bytes(listed.data(), listed.size());
-  Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
-  const Tensor scratch = Scratch(nbytes, first);
+  Tensor norm = at::empty({}, first->options().dtype(at::kFloat));
+  const Tensor scratch = Scratch(nbytes, *first);
   Launched(clip ? ugk_grad_clip(listed.data(), listed.size(), max_norm, Data(scratch), nbytes, norm.data_ptr<float>(), on.stream)
                 : ugk_grad_norm(listed.data(), listed.size(), Data(scratch), nbytes, norm.data_ptr<float>(), on.stream));
   return Wrap(std::move(norm));

@@ -86,7 +86,7 @@ struct Clear {
   uint64_t bytes;  // a whole number of elements
   uint32_t first;  // the launch's first block of kClearBytes
 };
-constexpr uint32_t kClearBytes = kSortBlock * 64;
+constexpr uint32_t kClearBytes = kSortBlock * 32;
 __device__ __forceinline__ void clear_block(const Clear &c, uint32_t block) {
   typedef typename ChunkOf<uint16_t, 8>::type chunk_t;
   const uint64_t base = ((uint64_t)c.first + block) * kClearBytes;

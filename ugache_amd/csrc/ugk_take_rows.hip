@@ -307,12 +307,13 @@ Plan plan_for(uint64_t rows) {
 }
 
 // Where some rows are named by nobody for certain the output is cleared on the side of the sort, which leaves the memory idle,
-// and only rows with entries are visited after it; where most may be named that would store them twice, but for outputs so
-// small that the launch which finds where rows begin costs more.  us, by position / by row: 16,384 entries over 50,000 bfloat16
-// rows of 2 KB 46 / 62, 40,000 over 50,000 76 / 98, 100,000 over 200,000 of 256 bytes 70 / 69; 3,000 over 3,000 of 128 bytes 18.6 /
-// 21.0, 10,000 over 5,000 of 256 bytes 30 / 31; 40,000 over 40,000 of 4 KB 145 / 111, 200,000 over 100,000 of 128 bytes 65 / 55,
-// 262,144 over 60,000 of 512 bytes 133 / 105.
-bool sums_by_row(size_t n, uint64_t rows, size_t dim) { return rows <= n && (n > 32768 || rows * dim > 4'000'000); }
+// and only rows with entries are visited after it; where most may be named that would store them twice, but for small outputs,
+// and a row's entries are found by a launch of its own instead of searches by whoever adds them.  us, by position / by row:
+// 16,384 entries over 50,000 bfloat16 rows of 2 KB 46 / 62, 40,000 over 50,000 76 / 98, 100,000 over 200,000 of 256 bytes 70 / 69;
+// 3,000 over 3,000 of 128 bytes 18.6 / 21.0, 10,000 over 5,000 of 256 bytes 30 / 31, 213,119 over as many of 16 bytes 37 / 42;
+// 40,000 over 40,000 of 4 KB 145 / 111, 262,144 over 60,000 of 512 bytes 133 / 105, 100,000 over 2,000 of 1 KB 59 / 48, 928,382 over
+// 42,603 of 8 bytes 84 / 70.
+bool sums_by_row(size_t n, uint64_t rows, size_t dim) { return rows <= n && (rows * dim > 4'000'000 || (n > 32768 && n > 2 * rows)); }
 
 // Entries a lane adds one after the other: few where the batch is small and their latency is what it costs, more where the
 // parts are traffic.  us, of 16 / 32 / 64: 16,384 bfloat16 rows of 1,024 elements 56 / 59 / 63, 30,000 95 / 95 / 104, 100,000 fp32
