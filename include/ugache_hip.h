@@ -477,7 +477,7 @@ int ugk_gather_scatter_staged_u32(const void *host_dev, uint64_t host_rows, cons
  *   slot_dev[i]                            the position of assignment i, -1 without an expert
  *   src_dev[p]                             the assignment at position p, -1 behind the last one
  * num_experts: 1 to 1024; n < 2^31.  The same ids give the same order on every run.  Few assignments need no workspace (0
- * bytes: workspace_dev may be NULL). */
+ * bytes: workspace_dev may be NULL); workspaces of this and the next operators are 8-byte aligned and need no clearing. */
 size_t ugk_expert_sort_workspace_bytes(size_t n, uint32_t num_experts);
 int ugk_expert_sort_i32(const int32_t *ids_dev, size_t n, uint32_t num_experts, int32_t *slot_dev, int32_t *src_dev,
                         int32_t *offsets_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
