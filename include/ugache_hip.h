@@ -188,8 +188,9 @@ int ugk_words_to_host_ticket(const uint32_t *a_dev, unsigned n_a, const uint32_t
                              uint32_t *dst_host, uint32_t value, unsigned spin_us, void *stream);
 /* The first launch of a kernel of one of this library's source files loads that file's code object onto the current
  * device, which takes 5 - 11 ms each the first time (a first gather of 51 MB: 12.4 ms, the second 0.9 ms).  This call
- * launches an empty kernel of every file on a stream of its own and waits for them, so that no later call pays; a
- * host library can make it from a helper thread while it is busy on the CPU. */
+ * launches an empty kernel of every file of the lookup path on a stream of its own and waits for them, so that no later call
+ * pays; a host library can make it from a helper thread while it is busy on the CPU.  The operators on rows (ugk_expert_*,
+ * ugk_take_rows*, ugk_grad_*) are not among them: three files of 0.3 - 2 ms, loaded by their first calls. */
 int ugk_preload_kernels(void);
 int ugk_device_sync(void);
 int ugk_event_create(void **event);

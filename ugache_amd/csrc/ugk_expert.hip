@@ -160,12 +160,6 @@ __global__ __launch_bounds__(kBlock) void combine_grad_kernel(const T *__restric
   }
 }
 
-__global__ void preload_expert_kernel() {}
-
-}  // namespace
-void preload_expert(hipStream_t stream) { hipLaunchKernelGGL(preload_expert_kernel, dim3(1), dim3(1), 0, stream); }
-
-namespace {
 
 template <typename K>
 int expert_sort(const K *ids, size_t n, uint32_t num_experts, int32_t *slot, int32_t *src, int32_t *offsets, void *workspace,

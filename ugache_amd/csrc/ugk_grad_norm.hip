@@ -201,12 +201,6 @@ __global__ __launch_bounds__(kBlock) void grad_scale_kernel(TensorList list, uin
   else scale_one<true, STREAM_OUT>(t, piece, factor, after);
 }
 
-__global__ void preload_grad_norm_kernel() {}
-
-}  // namespace
-void preload_grad_norm(hipStream_t stream) { hipLaunchKernelGGL(preload_grad_norm_kernel, dim3(1), dim3(1), 0, stream); }
-
-namespace {
 
 // calls launch(list, pieces before it) for the parts of the tensors in lists that fit a launch's arguments, from the last part
 // to the first where `backwards`

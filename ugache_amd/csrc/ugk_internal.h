@@ -96,16 +96,13 @@ __device__ __forceinline__ unsigned lane_id() { return __lane_id(); }
 // number of the wavefront in its workgroup, in a scalar register: what is computed from it stays scalar
 __device__ __forceinline__ unsigned wave_in_block() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
 
-// one per source file with kernels: launches an empty kernel of that file on `stream`
-void preload_expert(hipStream_t stream);
+// one per source file with kernels of the lookup path: launches an empty kernel of that file on `stream`
 void preload_gather(hipStream_t stream);
-void preload_grad_norm(hipStream_t stream);
 void preload_hotness(hipStream_t stream);
 void preload_partition(hipStream_t stream);
 void preload_pool(hipStream_t stream);
 void preload_pool_i64(hipStream_t stream);
 void preload_refresh(hipStream_t stream);
 void preload_table(hipStream_t stream);
-void preload_take_rows(hipStream_t stream);
 
 }  // namespace ugk

@@ -350,9 +350,6 @@ int ugk_preload_kernels(void) {
   ugk::preload_pool_i64(st);
   ugk::preload_refresh(st);
   ugk::preload_table(st);
-  ugk::preload_expert(st);
-  ugk::preload_take_rows(st);
-  ugk::preload_grad_norm(st);
   const hipError_t launched = hipGetLastError();
   const hipError_t waited = hipStreamSynchronize(st);
   (void)hipStreamDestroy(st);

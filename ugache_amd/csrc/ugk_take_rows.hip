@@ -269,12 +269,6 @@ __global__ __launch_bounds__(kBlock) void row_join_kernel(Sorted s, uint32_t run
 // more of the output than the sort's launches clear on their side
 __global__ __launch_bounds__(kSortBlock) void clear_kernel(Clear clear) { clear_block(clear, blockIdx.x); }
 
-__global__ void preload_take_rows_kernel() {}
-
-}  // namespace
-void preload_take_rows(hipStream_t stream) { hipLaunchKernelGGL(preload_take_rows_kernel, dim3(1), dim3(1), 0, stream); }
-
-namespace {
 
 template <typename I>
 int take_rows(const void *table, uint64_t num_rows, size_t stride, const I *index, size_t n, size_t dim, int elem, void *out, void *stream) {
