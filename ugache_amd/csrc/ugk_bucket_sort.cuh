@@ -360,7 +360,9 @@ static inline uint32_t bits_for(uint64_t values) {  // that tell `values` number
 // How a pass goes by its size.  Small tiles spread a batch over the chip, large ones keep the counts of all tiles few.  us of a
 // sort, entries per lane 2 / 4 / 8: 96,000 entries in 64 buckets 10.5 / 11.2 / 14.4, 480,000 11.6 / 11.9 / 15.1, 480,000 in 1,000
 // 23.0 / 18.7 / 20.3, 1 M in 128 18.1 / 15.8 / 17.2, two passes of 1 M over 1,024 124 / 107 / 97; 32,000 in 64, counts of the
-// tiles added up by every workgroup / by a launch of their own 8.5 / 10.5, 64,000 10.3 / 10.4.
+// tiles added up by every workgroup / by a launch of their own 8.5 / 10.5, 64,000 10.3 / 10.4.  Up to 4,096 entries are one tile: 1,200
+// take 5.4 in one launch of four entries a lane and 7.6 in one of eight or in two launches; 4,000 take 9.5 in one and 8.6 in
+// two, but a launch is 2.3 us of the host's time.
 struct SortShape {
   int items;
   Reach reach;

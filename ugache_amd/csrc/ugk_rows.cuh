@@ -108,7 +108,8 @@ static inline int for_rows(int elem, size_t dim, F f) {
   if (elem == 2) return dim >= 8 ? f(half_t(), std::integral_constant<int, 8>()) : f(half_t(), std::integral_constant<int, 1>());
   return dim >= 8 ? f(bhalf_t(), std::integral_constant<int, 8>()) : f(bhalf_t(), std::integral_constant<int, 1>());
 }
-// ... and whether so many of them are more than the memory-side cache holds
+// ... and whether so many of them are more than the memory-side cache holds (us, past the caches / the ordinary way: the sums of
+// 131,072 rows of 4 KB, 537 MB, 103 / 162; two passes over 12,297 rows of 4 KB, 49 MB, 37 / 32)
 template <typename F>
 static inline int for_rows_streamed(int elem, size_t dim, size_t rows, F f) {
   return for_rows(elem, dim, [&](auto type, auto vec) -> int {
@@ -116,7 +117,8 @@ static inline int for_rows_streamed(int elem, size_t dim, size_t rows, F f) {
   });
 }
 // ... for kernels that move elements of two or four bytes without looking at them, and whether their output of so many rows is
-// stored past the caches
+// stored past the caches (49,152 rows of 4 KB, 201 MB, past the caches / the ordinary way 40 / 36 us; 131,072, and their gradient
+// behind them, 224 / 259)
 template <typename F>
 static inline int for_moved_rows(int elem, size_t dim, size_t out_rows, F f) {
   const auto stored = [&](auto type, auto vec) -> int {
