@@ -79,8 +79,8 @@ __device__ __forceinline__ V block_before(V v, V &total, V *wave_sum) {
 }
 
 // Memory that has to be zero before the launch behind the sort, cleared by workgroups that the sort's launches have beside
-// those of the tiles: a sort of few entries leaves the memory and most of the chip alone.  Past the
-// caches, which the sort and the sums behind it need (us, 16,384 entries over 50,000 rows of 2 KB: 56 -> 46).
+// those of the tiles: a sort of few entries leaves the memory and most of the chip alone.  Past
+// the caches, which the sort and the sums behind it need (us, 16,384 entries over 50,000 rows of 2 KB: 56 -> 46).
 struct Clear {
   char *to;        // at any element's address
   uint64_t bytes;  // a whole number of elements
