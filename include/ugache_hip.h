@@ -533,7 +533,8 @@ typedef struct {
 } ugk_tensor_t;
 /* norm:  *norm_dev = sqrt of the sum of the squares of all elements of all tensors, squares and sums held in 64 bits.
  * clip:  the norm, and every element multiplied by min(1, max_norm / (norm + 1e-6)), rounded once.  A norm that is no number
- *        makes every element none; an infinite one makes the finite elements zero.
+ *        makes every element none; an infinite one makes the finite elements zero.  max_norm
+ *        infinite: nothing is scaled, whatever the norm is.
  * The tensors do not overlap one another's outputs.  The same gradients give the same bits on every run. */
 size_t ugk_grad_norm_workspace_bytes(const ugk_tensor_t *tensors, size_t n);
 int ugk_grad_norm(const ugk_tensor_t *tensors, size_t n, void *workspace_dev, size_t workspace_bytes, float *norm_dev, void *stream);

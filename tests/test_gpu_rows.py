@@ -6,6 +6,7 @@ by at most u relative to the value, for float16 at most 2^-25 absolute among its
 at most n * 2^-24 * sum |term| whatever its order, and a fused multiply-add adds one rounding.  Moved rows, positions and
 counts are equal bit for bit."""
 import os
+import subprocess
 import sys
 
 import numpy as np
@@ -560,6 +561,70 @@ def test_clipping_counts_as_a_change():
     assert to._version > before
 
 
+def test_gradients_from_a_generator():
+    g = gen(35)
+    grads = [randn(g, 50), randn(g, 7, 3, dtype=torch.bfloat16)]
+    before = [t.clone() for t in grads]
+    check_norm(co.coll_torch_grad_norm(t for t in grads), before)
+    check_norm(co.coll_torch_clip_grad_norm((t for t in grads), 0.5), before)
+    check_clipped(grads, before, 0.5)
+    out = [torch.empty_like(t) for t in grads]
+    co.coll_torch_clip_grad_norm((t for t in before), 0.25, out=(t for t in out))
+    check_clipped(out, before, 0.25)
+
+
+def test_gradients_that_share_memory_are_refused():
+    g = gen(36)
+    a, b = randn(g, 64), randn(g, 64)
+    before = a.clone()
+    free = torch.empty(256, device="cuda")
+    for grads, out in [([a[:40], a[39:]], None), ([b, a[8:16], a], None),       # scaled in place, one inside another
+                       ([a, b], [free[:64], free[63:127]]),                     # written to overlapping places
+                       ([a, b], [b, free[:64]]), ([a[:32], a[32:]], [a[16:48], free[:32]]),  # another's, or its own shifted
+                       ([a[:32]], [a[16:48]])]:
+        with pytest.raises(ValueError, match="same place"):
+            co.coll_torch_clip_grad_norm(grads, 1.0, out=out)
+    assert torch.equal(a, before)
+    # side by side, read twice, and into its own place
+    whole = torch.cat([a, b])
+    co.coll_torch_clip_grad_norm([a[:31], b, a[31:]], 0.5)
+    check_clipped([torch.cat([a, b])], [whole], 0.5)
+    co.coll_torch_clip_grad_norm([b, b], 0.25, out=[free[:64], free[64:128]])
+    check_clipped([free[:128]], [torch.cat([b, b])], 0.25)
+    before = [b.clone(), a.clone()]
+    co.coll_torch_clip_grad_norm([b, a], 0.125, out=[b, free[:64]])
+    check_clipped([b, free[:64]], before, 0.125)
+
+
+def test_clipping_without_a_limit():
+    g = gen(37)
+    for bad in (None, float("inf"), float("nan")):
+        grads = [randn(g, 90), randn(g, 30, dtype=torch.float16)]
+        if bad is not None:
+            grads[0][4] = bad
+        before = [t.clone() for t in grads]
+        out = [torch.empty_like(t) for t in grads]
+        for to in (out, None):
+            norm = co.coll_torch_clip_grad_norm(grads, float("inf"), out=to)
+            assert bool(torch.isfinite(norm)) == (bad is None)
+        for t, u, v in zip(grads, out, before):
+            assert torch.equal(t.nan_to_num(7.0), v.nan_to_num(7.0)) and torch.equal(u.nan_to_num(7.0), v.nan_to_num(7.0))
+
+
+def test_tensors_that_torch_holds_negated():
+    g = gen(38)
+    part = torch.complex(randn(g, 24, 1), randn(g, 24, 1)).conj().imag  # rows of one element, two apart, negated when read
+    assert part.is_neg()
+    index = torch.arange(24, device="cuda")
+    assert torch.equal(co.coll_torch_take_rows(part, index), part.resolve_neg())
+    one = part[:1, 0]
+    out = [torch.empty(1, device="cuda")]
+    co.coll_torch_clip_grad_norm([one], 1e9, out=out)
+    assert torch.equal(out[0], one.resolve_neg())
+    with pytest.raises(ValueError, match="in place"):
+        co.coll_torch_clip_grad_norm([one], 1.0)
+
+
 def test_norm_of_other_layouts():
     g = gen(34)
     a, b = randn(g, 40, 30), randn(g, 6, 5, 4, dtype=torch.float16)
@@ -626,6 +691,81 @@ def test_operators_replayed_from_two_graphs_as_eager(tokens):
             torch.cuda.synchronize()
             for a, b in zip(outs, eager):
                 assert torch.equal(a, b)
+
+
+def test_a_backward_pass_replayed():
+    """forward and backward through autograd in a graph, replayed on new inputs with eager steps between"""
+    tokens, top, experts, dim = 300, 2, 8, 40
+    g = gen(70)
+    table = randn(g, 500, dim, dtype=torch.bfloat16)
+    static = [torch.empty(tokens, dtype=torch.int64, device="cuda"), torch.empty(tokens, top, dtype=torch.int64, device="cuda"),
+              torch.empty(tokens, top, device="cuda", requires_grad=True), torch.empty(tokens, dim, dtype=torch.bfloat16, device="cuda")]
+
+    def fresh(seed):
+        f = gen(seed)
+        return [torch.randint(-1, 500, (tokens,), device="cuda", generator=f), random_ids(f, tokens, top, experts, 0.1),
+                torch.rand(tokens, top, device="cuda", generator=f).requires_grad_(), randn(f, tokens, dim, dtype=torch.bfloat16)]
+
+    def step(ids, chosen, w, grad):
+        leaf = table.detach().requires_grad_()
+        order = co.coll_torch_expert_sort(chosen, experts)
+        rows = co.coll_torch_expert_dispatch(co.coll_torch_take_rows(leaf, ids), order)
+        out = co.coll_torch_expert_combine(rows, order, w)
+        return [out.detach()] + list(torch.autograd.grad(out, [leaf, w], grad))
+
+    def fill(seed):
+        with torch.no_grad():
+            for to, t in zip(static, fresh(seed)):
+                to.copy_(t)
+
+    fill(71)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(*static)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*static)
+    for seed in range(72, 76):
+        fill(seed)
+        graph.replay()
+        eager = step(*fresh(seed))
+        torch.cuda.synchronize()
+        for a, b in zip(outs, eager):
+            assert torch.equal(a, b)
+
+
+def test_the_first_calls_of_a_process_captured():
+    """the kernels are loaded with their first call: that may be one that is recorded"""
+    code = """
+import sys
+import torch
+sys.path.insert(0, "ugache_amd")
+import collcache.torch as co
+x = torch.randn(64, 32, device="cuda")
+ids = torch.randint(0, 4, (64, 2), device="cuda")
+index = torch.randint(0, 64, (100,), device="cuda")
+def step():
+    order = co.coll_torch_expert_sort(ids, 4)
+    rows = co.coll_torch_expert_dispatch(x, order)
+    out = co.coll_torch_expert_combine(rows, order)
+    grad, _ = co.coll_torch_expert_combine_grad(out, rows, order)
+    taken = co.coll_torch_take_rows_grad(co.coll_torch_take_rows(x, index), index, 64)
+    clipped = torch.empty_like(taken)
+    return [out, grad, taken, co.coll_torch_clip_grad_norm([taken], 1.0, out=[clipped]), clipped]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = step()
+for _ in range(3):
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, step()))
+print("replayed", flush=True)
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "replayed" in done.stdout, done.stderr[-2000:]
 
 
 def test_operators_on_two_streams_at_once():

@@ -140,7 +140,8 @@ def coll_torch_take_rows_grad(grad, index, num_rows):
 
 def coll_torch_grad_norm(grads):
     """the l2 norm over all elements of all tensors: a float32 GPU scalar.  Squares and sums are held in 64 bits, so neither
-    large nor tiny gradients leave the range.  grads: a tensor or a sequence of them; entries that are None are left out."""
+    large nor tiny gradients leave the range.  grads: a tensor, or a sequence or an iterator of them; entries that are None are
+    left out."""
     return _native.grad_norm(grads, None, None)
 
 
@@ -148,6 +149,7 @@ def coll_torch_clip_grad_norm(grads, max_norm, out=None):
     """scale the gradients so that their norm is at most max_norm: every element times min(1, max_norm / (norm + 1e-6)), rounded
     once; returns the norm before that, a float32 GPU scalar.  In place, or into the tensors of `out` (the gradients then
     stay).  Without a host wait: a norm that is not finite shows in the result (no number: every element none; infinite: the
-    finite elements zero).  No two gradients may share memory.  Gradients of equal keys have to be summed before
+    finite elements zero); max_norm infinite: nothing is scaled.  What is written is written once and is no other gradient's
+    memory: ValueError.  Gradients of equal keys have to be summed before
     (coll_torch_take_rows_grad): the norm of the parts is not the norm of the sum."""
     return _native.grad_norm(grads, float(max_norm), out)

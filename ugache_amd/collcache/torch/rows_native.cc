@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cstdint>
 #include <string>
 #include <vector>
 
@@ -44,7 +45,7 @@ Tensor Unpack(const char *what, py::handle h, Kind kind, int dev = -1) {
   const bool right = kind == kRowsKind ? ElemOf(t) != 0 : kind == kIntKind ? IsInt(t) : t.scalar_type() == ScalarType::Int;
   if (!t.is_cuda() || t.layout() != c10::kStrided || !right) throw py::type_error(std::string(what) + " must be a GPU tensor of " + types);
   if (dev >= 0 && t.get_device() != dev) throw py::value_error(std::string(what) + " must be on the GPU of the other tensors");
-  return t;
+  return t.is_neg() ? t.resolve_neg() : t;  // memory that torch holds negated until it is read
 }
 
 // enqueues on torch's current stream of GPU `dev`, which is the current device while the call runs
@@ -235,10 +236,11 @@ py::object TakeRowsGrad(py::handle grad_h, py::handle index_h, int64_t num_rows)
   return Wrap(std::move(out));
 }
 
-// a sequence of tensors, or one tensor, held while the call runs
+// the tensors of a sequence or an iterator, or one tensor, or none of them, held while the call runs
 class Items {
  public:
   explicit Items(py::handle h) {
+    if (h.is_none()) return;
     if (THPVariable_Check(h.ptr())) {
       _one = h.ptr();
       return;
@@ -246,7 +248,7 @@ class Items {
     _seq = py::reinterpret_steal<py::object>(PySequence_Fast(h.ptr(), "gradients must be a tensor or a sequence of tensors"));
     if (!_seq) throw py::error_already_set();
   }
-  size_t size() const { return _one ? 1 : (size_t)PySequence_Fast_GET_SIZE(_seq.ptr()); }
+  size_t size() const { return _one ? 1 : !_seq ? 0 : (size_t)PySequence_Fast_GET_SIZE(_seq.ptr()); }
   PyObject *operator[](size_t i) const { return _one ? _one : PySequence_Fast_GET_ITEM(_seq.ptr(), (Py_ssize_t)i); }
 
  private:
@@ -262,6 +264,27 @@ const Tensor &ListedTensor(const char *what, PyObject *o, int dev) {
   return *t;
 }
 
+struct Span {
+  uintptr_t from, to;
+  Span(const void *at, size_t nbytes) : from((uintptr_t)at), to((uintptr_t)at + nbytes) {}
+};
+// what is written is written once, and is nothing that the call reads but its own gradient; read[i] goes with written[i],
+// or is left out where it is that place
+void CheckPlaces(const std::vector<Span> &read, std::vector<Span> written) {
+  std::vector<Span> elsewhere;
+  for (size_t i = 0; i < read.size(); ++i)
+    if (read[i].from != written[i].from) elsewhere.push_back(read[i]);
+  std::sort(written.begin(), written.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].from < written[i - 1].to) throw py::value_error("two gradients are written to the same place");
+  for (const Span &r : elsewhere) {
+    // the first that ends behind the start of r
+    const auto w = std::upper_bound(written.begin(), written.end(), r.from, [](uintptr_t at, const Span &s) { return at < s.to; });
+    if (w != written.end() && w->from < r.to)
+      throw py::value_error("an output is in the same place as another gradient, or as a part of its own");
+  }
+}
+
 // max_norm None: the norm alone; out None: in place
 py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h) {
   const bool clip = !max_norm_h.is_none(), elsewhere = !out_h.is_none();
@@ -270,15 +293,18 @@ py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h)
     max_norm = max_norm_h.cast<double>();
     if (!(max_norm >= 0)) throw py::value_error("max_norm must be at least 0, got " + std::to_string(max_norm));
   }
-  const Items grads(grads_h), outs(elsewhere ? out_h : grads_h);
+  const Items grads(grads_h);  // once: it may be an iterator
+  const Items outs(elsewhere ? out_h : py::handle(Py_None));
   const size_t n = grads.size();
-  if (outs.size() != n) throw py::value_error(std::to_string(outs.size()) + " outputs for " + std::to_string(n) + " gradients");
+  if (elsewhere && outs.size() != n)
+    throw py::value_error(std::to_string(outs.size()) + " outputs for " + std::to_string(n) + " gradients");
   std::vector<ugk_tensor_t> listed;
   std::vector<Tensor> copies;
-  std::vector<const void *> written;
+  std::vector<Span> read, written;
   std::vector<c10::TensorImpl *> changed;
   listed.reserve(n);
-  written.reserve(n);
+  if (clip) written.reserve(n);
+  if (clip && elsewhere) read.reserve(n);
   changed.reserve(n);
   const Tensor *first = nullptr;
   int dev = -1;
@@ -287,17 +313,17 @@ py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h)
     const Tensor *g = &ListedTensor("a gradient", grads[i], dev);
     if (!first) first = g, dev = (int)g->get_device();
     // in place and for the norm alone the order of the elements is nobody's matter, so long as they are one run of memory
-    if (!g->is_contiguous() && (elsewhere || !g->is_non_overlapping_and_dense())) {
+    if (g->is_neg() || (!g->is_contiguous() && (elsewhere || !g->is_non_overlapping_and_dense()))) {
       if (clip && !elsewhere && g->numel())
         throw py::value_error("a gradient whose elements are no run of memory cannot be scaled in place");
-      copies.push_back(g->contiguous());
+      copies.push_back(g->resolve_neg().contiguous());
       g = nullptr;
     }
     const Tensor &from = g ? *g : copies.back();
     void *at = from.data_ptr(), *to = at;
     if (elsewhere) {
       const Tensor &o = ListedTensor("an output", outs[i], dev);
-      if (o.scalar_type() != from.scalar_type() || o.sizes() != from.sizes() || !o.is_contiguous())
+      if (o.scalar_type() != from.scalar_type() || o.sizes() != from.sizes() || !o.is_contiguous() || o.is_neg())
         throw py::value_error("an output must be contiguous and of its gradient's shape, type and GPU");
       to = o.data_ptr();
       changed.push_back(o.unsafeGetTensorImpl());
@@ -305,12 +331,11 @@ py::object GradNorm(py::handle grads_h, py::handle max_norm_h, py::handle out_h)
       changed.push_back(from.unsafeGetTensorImpl());
     }
     listed.push_back(ugk_tensor_t{at, to, (uint64_t)from.numel(), ElemOf(from), 0});
-    if (clip && from.numel()) written.push_back(to);
+    if (clip && from.numel()) written.push_back(Span(to, from.nbytes()));
+    if (clip && elsewhere && from.numel()) read.push_back(Span(at, from.nbytes()));
   }
   if (!first) throw py::value_error("no gradients");
-  std::sort(written.begin(), written.end());
-  if (std::adjacent_find(written.begin(), written.end()) != written.end())
-    throw py::value_error("two gradients are written to the same place");
+  CheckPlaces(read, written);
   const On on(*first);
   for (c10::TensorImpl *t : changed) t->bump_version();  // what autograd has saved of them is stale
   const size_t nbytes = ugk_grad_norm_workspace_bytes(listed.data(), listed.size());

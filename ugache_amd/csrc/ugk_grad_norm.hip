@@ -177,7 +177,7 @@ __device__ __forceinline__ void scale_one(const Listed &t, uint32_t piece, float
 }
 
 // out = data * min(1, max_norm / (norm + 1e-6)), rounded once; nothing to do in place where the factor is 1.  A norm that is
-// no number makes every element none.
+// no number makes every element none.  An infinite max_norm scales nothing, whatever the norm is.
 // The first `kept` pieces are read the ordinary way.  Few pieces are added up by every workgroup, and the norm is left by the
 // first, without a launch in between (`norm` set; 98,816 gradients in twelve tensors: 9.0 -> 7.3 us); the sum of more is in
 // total[0], in front of the pieces'.
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kBlock) void grad_scale_kernel(TensorList list, uin
                                                             float *__restrict__ norm, double max_norm) {
   const double length = sqrt(norm ? sum_of_pieces<kBlock>(total + 1, pieces) : *total);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)length;  // the same in every list
-  const double ratio = max_norm / (length + 1e-6);
+  const double ratio = isinf(max_norm) ? 1.0 : max_norm / (length + 1e-6);
   // a factor near the end of float's range, which a norm beyond it brings, would lose its digits: it is multiplied in two steps
   const bool small = ratio < 0x1p-100;
   const float factor = ratio >= 1.0 ? 1.f : (float)(small ? ratio * 0x1p100 : ratio), after = small ? 0x1p-100f : 1.f;
