@@ -1,0 +1,85 @@
+"""GPU tests of calls of the operators on rows (collcache.torch) that a program can make beside the ordinary ones: forward-mode
+tensors, shapes that pair rows with other entries, tensors changed or let go between a forward and a backward pass, rows that
+very many entries name.
+
+Small whole numbers are summed exactly in float32 as long as no partial sum passes 2^24: results are then equal bit for bit
+whatever the order, and one entry lost or counted twice shows."""
+import os
+import sys
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "ugache_amd"))
+
+if torch.cuda.is_available():
+    import collcache.torch as co
+    import torch.autograd.forward_ad as forward_ad
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, device="cuda", generator=g, dtype=dtype)
+
+
+def whole(g, *shape, dtype=torch.float32):
+    return torch.randint(-3, 4, shape, device="cuda", generator=g).to(dtype)
+
+
+def order_of(g, tokens, top, experts):
+    ids = torch.topk(torch.rand(tokens, experts, device="cuda", generator=g), top, dim=1).indices
+    return co.coll_torch_expert_sort(ids, experts)
+
+
+# ---- forward mode ---------------------------------------------------------------------------------------------------
+
+
+def test_a_tangent_is_refused_and_not_lost():
+    g = gen(1)
+    order = order_of(g, 10, 2, 4)
+    x, rows, w, table = randn(g, 10, 8), randn(g, 20, 8), torch.rand(10, 2, device="cuda", generator=g), randn(g, 30, 8)
+    index = torch.randint(0, 30, (12,), device="cuda", generator=g)
+    out = [torch.empty_like(x)]
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: co.coll_torch_expert_dispatch(dual(x), order), lambda: co.coll_torch_expert_combine(dual(rows), order, w),
+                     lambda: co.coll_torch_expert_combine(rows, order, dual(w)), lambda: co.coll_torch_take_rows(dual(table), index),
+                     lambda: co.coll_torch_expert_dispatch(dual(x.clone().requires_grad_()), order),
+                     lambda: co.coll_torch_take_rows(dual(table.clone().requires_grad_()), index),
+                     lambda: co.coll_torch_expert_dispatch_grad(dual(rows), order), lambda: co.coll_torch_take_rows_grad(dual(x), index[:10], 30),
+                     lambda: co.coll_torch_expert_combine_grad(x, dual(rows), order, w), lambda: co.coll_torch_grad_norm([x, dual(rows)]),
+                     lambda: co.coll_torch_clip_grad_norm([dual(x)], 1.0, out=out), lambda: co.coll_torch_clip_grad_norm([x], 1.0, out=[dual(out[0])])):
+            with pytest.raises(NotImplementedError):
+                call()
+        # tensors without a tangent are nothing to forward mode
+        assert torch.equal(co.coll_torch_take_rows(table, index), table[index])
+        assert torch.equal(co.coll_torch_take_rows(forward_ad.unpack_dual(dual(table)).primal, index), table[index])
+    assert torch.equal(co.coll_torch_take_rows(table, index), table[index])
+
+
+def test_a_function_with_a_forward_mode_of_its_own():
+    """the operator is linear: a program can give it its tangent"""
+    class Take(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, table, index):
+            ctx.index = index
+            return co.coll_torch_take_rows(table, index)
+
+        @staticmethod
+        def jvp(ctx, tangent, _):
+            return co.coll_torch_take_rows(tangent, ctx.index)
+
+    g = gen(2)
+    table, tangent, index = randn(g, 30, 8), randn(g, 30, 8), torch.randint(0, 30, (12,), device="cuda", generator=g)
+    with forward_ad.dual_level():
+        got = forward_ad.unpack_dual(Take.apply(forward_ad.make_dual(table, tangent), index))
+        assert torch.equal(got.primal, table[index]) and torch.equal(got.tangent, tangent[index])

@@ -7,9 +7,10 @@ inputs give the same bits.  Every call takes its memory from torch, so calls on 
 HIP graphs share nothing.  What cannot be computed raises TypeError or ValueError before anything is enqueued; a failing
 launch raises RuntimeError.
 
-The operators that have a gradient record it (torch.autograd) where an input asks for one; the gradients are entry points of
-their own as well, for programs that call backward passes themselves.  The calls themselves are compiled
-(collcache.torch.rows_native).
+The operators that are called differentiable below record their gradient (torch.autograd, reverse mode) where an input asks
+for one; the gradients are entry points of their own as well, for programs that call backward passes themselves, and record
+nothing, like the norm and the clipping.  There is no forward mode: a tensor with a tangent (torch.autograd.forward_ad) raises
+NotImplementedError.  The calls themselves are compiled (collcache.torch.rows_native).
 """
 import collections
 

@@ -5,6 +5,7 @@
 // Tensors are torch's own (ATen); the raw stream comes from torch through its Python function, so that no HIP header is
 // needed.  Built by python -m ugache_amd.build; collcache.torch.rows is the public face and documents the calls.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
@@ -37,11 +38,21 @@ int ElemOf(const Tensor &t) {  // 0: none of the three
 }
 bool IsInt(const Tensor &t) { return t.scalar_type() == ScalarType::Int || t.scalar_type() == ScalarType::Long; }
 
+// The operators have no forward-mode derivative: a tangent is refused instead of left out of the result, which would make the
+// derivative zero without a word.  (Not where torch has forward mode switched off: inside a Function that brings its own.)
+void NoTangent(const char *what, const Tensor &t) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined()) return;
+  PyErr_SetString(PyExc_NotImplementedError,
+                  (std::string(what) + " has a tangent: the operators on rows have no forward-mode derivative").c_str());
+  throw py::error_already_set();
+}
+
 enum Kind { kRowsKind, kIntKind, kInt32Kind };
 Tensor Unpack(const char *what, py::handle h, Kind kind, int dev = -1) {
   const char *types = kind == kRowsKind ? "float32, float16, bfloat16" : kind == kIntKind ? "int32, int64" : "int32";
   if (!THPVariable_Check(h.ptr())) throw py::type_error(std::string(what) + " must be a GPU tensor of " + types);
   const Tensor &t = THPVariable_Unpack(h.ptr());
+  NoTangent(what, t);
   const bool right = kind == kRowsKind ? ElemOf(t) != 0 : kind == kIntKind ? IsInt(t) : t.scalar_type() == ScalarType::Int;
   if (!t.is_cuda() || t.layout() != c10::kStrided || !right) throw py::type_error(std::string(what) + " must be a GPU tensor of " + types);
   if (dev >= 0 && t.get_device() != dev) throw py::value_error(std::string(what) + " must be on the GPU of the other tensors");
@@ -258,6 +269,7 @@ class Items {
 
 const Tensor &ListedTensor(const char *what, PyObject *o, int dev) {
   const Tensor *t = THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+  if (t) NoTangent(what, *t);
   if (!t || !t->is_cuda() || t->layout() != c10::kStrided || ElemOf(*t) == 0)
     throw py::type_error(std::string(what) + " must be a GPU tensor of float32, float16, bfloat16");
   if (dev >= 0 && t->get_device() != dev) throw py::value_error(std::string(what) + " must be on the GPU of the other tensors");
