@@ -4,9 +4,13 @@ very many entries name.
 
 Small whole numbers are summed exactly in float32 as long as no partial sum passes 2^24: results are then equal bit for bit
 whatever the order, and one entry lost or counted twice shows."""
+import json
 import os
+import shutil
+import subprocess
 import sys
 
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +87,50 @@ def test_a_function_with_a_forward_mode_of_its_own():
     with forward_ad.dual_level():
         got = forward_ad.unpack_dual(Take.apply(forward_ad.make_dual(table, tangent), index))
         assert torch.equal(got.primal, table[index]) and torch.equal(got.tangent, tangent[index])
+
+
+# ---- the package without the compiled module ------------------------------------------------------------------------
+
+LAYER = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import numpy as np, torch
+import collcache.torch as co
+import collcache.torch.serving as hps
+from collcache.torch import rows
+assert co.__file__.startswith(sys.argv[1])
+assert hps.Config(ps_config_file=sys.argv[2]) == "OK"
+g = torch.Generator().manual_seed(3)
+hps.record_hotness(torch.randint(0, 2000, (5000,), generator=g).cuda())
+assert hps.Init(ps_config_file=sys.argv[2], global_batch_size=256) == "OK"
+ids = torch.randint(0, 2000, (300, 4), generator=g)
+at = torch.stack([torch.arange(300).repeat_interleave(4), torch.arange(4).repeat(300)])
+sp = torch.sparse_coo_tensor(at, ids.reshape(-1), (300, 4)).cuda()
+want = torch.from_numpy(np.fromfile(sys.argv[3], dtype=np.float32)).view(2000, 16)[ids]
+for in_library in (False, True):
+    layer = hps.SparseLookupLayer(model_name="dlrm", table_id=0, emb_vec_size=16, unique_in_library=in_library)
+    assert torch.equal(layer(sp, combiner="sum").cpu(), want.sum(1))
+print("operators" if rows.AVAILABLE else "none", flush=True)
+hps.Shutdown()
+"""
+
+
+@pytest.mark.parametrize("module", ["there", "absent"])
+def test_the_sparse_layer_without_the_compiled_module(tmp_path, module):
+    package = os.path.join(ROOT, "ugache_amd")
+    if module == "absent":
+        package = str(tmp_path / "ugache_amd")
+        shutil.copytree(os.path.join(ROOT, "ugache_amd"), package, copy_function=os.symlink,
+                        ignore=shutil.ignore_patterns("__pycache__", "_build", "csrc", "rows_native.*"))
+    model = tmp_path / "dlrm_sparse.model"
+    model.mkdir()
+    np.arange(2000, dtype=np.int64).tofile(model / "key")
+    np.random.default_rng(1).integers(-9, 10, (2000, 16)).astype(np.float32).tofile(model / "emb_vector")
+    path = tmp_path / "ps_config.json"
+    path.write_text(json.dumps({"iteration_per_epoch": 50, "epoch": 1, "coll_cache_enable_refresh": False, "models": [{
+        "model": "dlrm", "sparse_files": [str(model)], "gpucacheper": 0.3, "max_batch_size": 4096, "deployed_device_list": [0],
+        "maxnum_catfeature_query_per_table_per_sample": [26], "embedding_vecsize_per_table": [16], "max_vocabulary_size": [2000]}]}))
+    done = subprocess.run([sys.executable, "-c", LAYER, package, str(path), str(model / "emb_vector")], cwd=tmp_path, capture_output=True,
+                          text=True, timeout=100)
+    assert done.returncode == 0, done.stderr[-2000:]
+    assert done.stdout.split()[-1] == ("operators" if module == "there" else "none")

@@ -1,5 +1,7 @@
 """CPU tests of the calls of the operators on rows (collcache.torch) that are turned down, or answered, before any GPU is asked."""
 import os
+import shutil
+import subprocess
 import sys
 
 import pytest
@@ -11,6 +13,7 @@ sys.path.insert(0, os.path.join(ROOT, "ugache_amd"))
 
 import collcache.torch as co  # noqa: E402
 import torch.autograd.forward_ad as forward_ad  # noqa: E402
+from ugache_amd import build  # noqa: E402
 
 ORDER = co.ExpertOrder(torch.zeros(4, 2, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), torch.zeros(5, dtype=torch.int32))
 
@@ -60,3 +63,37 @@ def test_what_has_no_tangent_of_its_own_is_taken():
         assert forward_ad.unpack_dual(Own.apply(dual)).tangent == 3
     with pytest.raises(TypeError, match="GPU"):
         co.coll_torch_grad_norm([dual])
+
+
+# ---- the package without the compiled module ------------------------------------------------------------------------
+
+WITHOUT = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+import collcache.torch as co
+import collcache.torch.serving as hps
+assert co.__file__.startswith(sys.argv[1]) and callable(co.coll_torch_lookup_unique)
+assert torch.equal(hps._at_positions(torch.arange(12.).view(4, 3), torch.tensor([2, 0], dtype=torch.int32)), torch.arange(12.).view(4, 3)[[2, 0]])
+for call in (lambda: co.coll_torch_expert_sort(torch.zeros(4, 2, dtype=torch.int64), 4), lambda: co.coll_torch_grad_norm([torch.zeros(3)]),
+             lambda: co.coll_torch_take_rows(torch.zeros(4, 8, requires_grad=True), torch.zeros(3, dtype=torch.int64))):
+    try:
+        call()
+    except ImportError as e:
+        assert "rows_native" in str(e) and "ugache_amd.build" in str(e), e
+    else:
+        raise AssertionError("no ImportError")
+print("went on")
+"""
+
+
+@pytest.mark.parametrize("module", ["absent", "not loadable"])
+def test_the_package_without_the_compiled_module(tmp_path, module):
+    """lookups need no rows_native: the package is imported without it, and the operators on rows say what they lack"""
+    copy = tmp_path / "ugache_amd"
+    shutil.copytree(os.path.join(ROOT, "ugache_amd"), copy, copy_function=os.symlink,
+                    ignore=shutil.ignore_patterns("__pycache__", "_build", "csrc", "rows_native.*"))
+    if module == "not loadable":
+        (copy / "collcache" / "torch" / os.path.basename(build.native_rows_path())).write_bytes(b"")
+    done = subprocess.run([sys.executable, "-c", WITHOUT, str(copy)], cwd=tmp_path, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "went on" in done.stdout, done.stderr[-2000:]

@@ -10,15 +10,31 @@ launch raises RuntimeError.
 The operators that are called differentiable below record their gradient (torch.autograd, reverse mode) where an input asks
 for one; the gradients are entry points of their own as well, for programs that call backward passes themselves, and record
 nothing, like the norm and the clipping.  There is no forward mode: a tensor with a tangent (torch.autograd.forward_ad) raises
-NotImplementedError.  The calls themselves are compiled (collcache.torch.rows_native).
+NotImplementedError.  The calls themselves are compiled (collcache.torch.rows_native); where that module is not built, or built
+for another torch, they raise ImportError and the lookups go on without them.
 """
 import collections
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import rows_native as _native
 
+class _Missing:
+    """in the place of the compiled module: every call of it raises why it could not be loaded"""
+
+    def __init__(self, why):
+        self._why = why
+
+    def __getattr__(self, name):
+        raise ImportError("the operators on rows need collcache.torch.rows_native (python -m ugache_amd.build): %s" % self._why)
+
+
+try:
+    from . import rows_native as _native
+except ImportError as _error:
+    _native = _Missing(_error)
+
+AVAILABLE = not isinstance(_native, _Missing)
 MAX_EXPERTS = 1024
 
 ExpertOrder = collections.namedtuple("ExpertOrder", ["slot", "src", "offsets"])

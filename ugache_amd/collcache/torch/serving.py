@@ -26,6 +26,7 @@ import torch
 
 from . import adapter as _adapter
 from . import c_lib as _c_lib
+from . import rows as _rows
 from ..common import _basics
 
 # the share of every batch whose hotness the serving loop records (lookup_manager.cc:295-300: the first 5 %)
@@ -189,6 +190,13 @@ class LookupLayer(torch.nn.Module):
         return emb.reshape(tuple(inputs.shape) + (self.emb_vec_size,))
 
 
+def _at_positions(rows, index):
+    """the rows of distinct ids, at the positions of a batch that name them"""
+    if _rows.AVAILABLE:
+        return _adapter.coll_torch_take_rows(rows, index)
+    return rows.index_select(0, index.long())
+
+
 class SparseLookupLayer(torch.nn.Module):
     """collcache_tf2.SparseLookupLayer (core/sparse_lookup_layer.py:27-265), i.e. embedding_lookup_sparse over the
     cache: `sp_ids` is an N x M sparse COO tensor of int64 ids in row-major order with at least one id per row,
@@ -233,10 +241,10 @@ class SparseLookupLayer(torch.nn.Module):
         if self.unique_in_library:  # unique + lookup in one call, the unique by the library's GPU hash set
             self.lookup.check(ids)
             emb_unique, idx = _adapter.coll_torch_lookup_unique(0, ids)
-            embeddings = _adapter.coll_torch_take_rows(emb_unique, idx)
+            embeddings = _at_positions(emb_unique, idx)
         else:
             ids, idx = torch.unique(ids, return_inverse=True)
-            embeddings = _adapter.coll_torch_take_rows(self.lookup(ids), idx)
+            embeddings = _at_positions(self.lookup(ids), idx)
         original_dtype = embeddings.dtype
         if embeddings.dtype in (torch.float16, torch.bfloat16):
             embeddings = embeddings.float()  # low-precision rows are combined in fp32
