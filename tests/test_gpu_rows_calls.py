@@ -134,3 +134,51 @@ def test_the_sparse_layer_without_the_compiled_module(tmp_path, module):
                           text=True, timeout=100)
     assert done.returncode == 0, done.stderr[-2000:]
     assert done.stdout.split()[-1] == ("operators" if module == "there" else "none")
+
+
+# ---- shapes that say which entry belongs to which ---------------------------------------------------------------------
+
+
+def test_weights_in_another_order_are_refused():
+    g = gen(4)
+    tokens, top = 12, 3
+    order = order_of(g, tokens, top, 5)
+    rows, w = randn(g, tokens * top, 8), torch.rand(tokens, top, device="cuda", generator=g)
+    grad = randn(g, tokens, 8)
+    want = co.coll_torch_expert_combine(rows, order, w)
+    want_grad = co.coll_torch_expert_combine_grad(grad, rows, order, w)[1]
+    for shape in ((tokens * top,), (4, 3, top), (tokens, top, 1), (1, tokens, top), (tokens * top, 1)):
+        assert torch.equal(co.coll_torch_expert_combine(rows, order, w.view(shape)), want)
+        got = co.coll_torch_expert_combine_grad(grad, rows, order, w.view(shape))[1]
+        assert got.shape == shape and torch.equal(got, want_grad.view(shape))
+    for bad in (w.t(), w.t().contiguous(), w.view(6, 6), w.t().unsqueeze(0), w.view(4, 3, top).transpose(1, 2).reshape(4, 9)):
+        for call in (lambda: co.coll_torch_expert_combine(rows, order, bad), lambda: co.coll_torch_expert_combine_grad(grad, rows, order, bad),
+                     lambda: co.coll_torch_expert_combine(rows, order, bad.detach().requires_grad_())):
+            with pytest.raises(ValueError, match="top_k"):
+                call()
+    # one expert a token, and one token: there is only one order
+    single = co.coll_torch_expert_sort(torch.arange(12, device="cuda") % 5, 5)
+    for shape in ((12,), (12, 1), (3, 4), (1, 12)):
+        assert torch.equal(co.coll_torch_expert_combine(rows[:12], single, w.reshape(-1)[:12].view(shape)),
+                           co.coll_torch_expert_combine(rows[:12], single, w.reshape(-1)[:12]))
+    alone = co.coll_torch_expert_sort(torch.arange(3, device="cuda").view(1, 3), 5)
+    for shape in ((3,), (1, 3), (3, 1)):
+        assert torch.equal(co.coll_torch_expert_combine(rows[:3], alone, w[0].view(shape)), co.coll_torch_expert_combine(rows[:3], alone, w[:1]))
+    none = co.coll_torch_expert_sort(torch.empty(0, 4, dtype=torch.int64, device="cuda"), 9)
+    assert co.coll_torch_expert_combine(rows[:0], none, torch.empty(4, 0, device="cuda")).shape == (0, 8)
+
+
+def test_a_gradient_in_another_order_than_its_index_is_refused():
+    g = gen(5)
+    index, grad = torch.randint(0, 9, (4, 6), device="cuda", generator=g), whole(g, 4, 6, 8)
+    want = torch.zeros(9, 8, device="cuda").index_add_(0, index.reshape(-1), grad.view(24, 8))
+    for i, d in ((index, grad), (index.view(24), grad), (index, grad.view(24, 8)), (index.view(2, 2, 6), grad.view(2, 2, 6, 8)),
+                 (index.unsqueeze(-1), grad), (index, grad.unsqueeze(0)), (index.view(1, 24), grad)):
+        assert torch.equal(co.coll_torch_take_rows_grad(d, i, 9), want)
+    for i, d in ((index.t(), grad), (index.t().contiguous(), grad), (index, grad.transpose(0, 1)), (index.view(2, 12), grad),
+                 (index.view(2, 2, 6), grad)):
+        with pytest.raises(ValueError, match="index.shape"):
+            co.coll_torch_take_rows_grad(d, i, 9)
+    one = co.coll_torch_take_rows_grad(grad[0, 0], index[0, 0], 9)
+    assert torch.equal(one[index[0, 0]], grad[0, 0]) and int(one.any(1).sum()) == int(grad[0, 0].any())
+    assert not co.coll_torch_take_rows_grad(grad[:0], index.t()[:, :0], 9).any()

@@ -118,8 +118,8 @@ def coll_torch_expert_dispatch_grad(grad_rows, order):
 def coll_torch_expert_combine(rows, order, weights=None):
     """what came back from the experts, added up per token: a new [tokens, dim] tensor, out[t] = sum over k of weights[t, k] *
     rows[order.slot[t, k]] in fp32; assignments without an expert add nothing, a token without any gives a zero row.
-    rows: [tokens * top_k, dim]; weights: float32, float16 or bfloat16, one per assignment, or None for ones.
-    Differentiable in rows and weights."""
+    rows: [tokens * top_k, dim]; weights: float32, float16 or bfloat16, [tokens, top_k] (or any leading shape of
+    that many tokens) or [tokens * top_k], or None for ones.  Differentiable in rows and weights."""
     if _grad_enabled() and (_asks(rows) or _asks(weights)):
         return _Combine.apply(rows, weights, order.slot, order.offsets)
     return _native.combine(rows, order.slot, order.offsets, weights)
@@ -147,8 +147,8 @@ def coll_torch_take_rows(table, index):
 def coll_torch_take_rows_grad(grad, index, num_rows):
     """the gradient of coll_torch_take_rows, or of any lookup of rows by key: a new [num_rows, dim] tensor whose row r is the
     sum of grad[i] over all i with index[i] == r, added in fp32 in an order that the index alone fixes; rows nobody named
-    are zero.  grad: [*index.shape, dim].  With the distinct keys and the inverse of coll_torch_lookup_unique: the gradient of
-    the distinct rows."""
+    are zero.  grad: [*index.shape, dim], or one of the two a list in the order of the other.  With the distinct keys and the
+    inverse of coll_torch_lookup_unique: the gradient of the distinct rows."""
     return _native.take_rows_grad(grad, index, num_rows)
 
 

@@ -5,6 +5,7 @@
 // Tensors are torch's own (ATen); the raw stream comes from torch through its Python function, so that no HIP header is
 // needed.  Built by python -m ugache_amd.build; collcache.torch.rows is the public face and documents the calls.
 #include <ATen/ATen.h>
+#include <ATen/core/DimVector.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <pybind11/pybind11.h>
@@ -13,6 +14,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <iterator>
 #include <string>
 #include <vector>
 
@@ -116,6 +118,13 @@ Order OrderOf(py::handle slot_h, py::handle offsets_h, int dev) {
   return o;
 }
 
+// sizes without those of one, which say nothing of the order
+at::DimVector Wide(at::IntArrayRef sizes) {
+  at::DimVector out;
+  std::copy_if(sizes.begin(), sizes.end(), std::back_inserter(out), [](int64_t n) { return n != 1; });
+  return out;
+}
+
 struct Weights {
   Tensor t;
   const void *data = nullptr;
@@ -127,6 +136,11 @@ Weights WeightsOf(py::handle h, const Order &o, int dev) {
   w.t = Unpack("weights", h, kRowsKind, dev).contiguous();
   if (w.t.numel() != o.n)
     throw py::value_error(std::to_string(w.t.numel()) + " weights for " + std::to_string(o.n) + " assignments");
+  // one after the other, or those of a token beside one another; any other shape has them in another order
+  const at::DimVector wide = Wide(w.t.sizes());
+  if (o.n && wide.size() > 1 && o.top > 1 && wide.back() != o.top)
+    throw py::value_error("weights must be shaped [tokens, top_k] or [tokens * top_k]: the last size is " + std::to_string(wide.back()) +
+                          ", top_k " + std::to_string(o.top));
   w.data = w.t.data_ptr();
   w.elem = ElemOf(w.t);
   return w;
@@ -232,6 +246,11 @@ py::object TakeRowsGrad(py::handle grad_h, py::handle index_h, int64_t num_rows)
   const Tensor index = Unpack("index", index_h, kIntKind, grad.t.get_device()).contiguous();
   const int64_t n = index.numel();
   if (grad.n != n) throw py::value_error(std::to_string(grad.n) + " rows for " + std::to_string(n) + " indices");
+  // of the index's shape, or one of the two is a list
+  const at::IntArrayRef of = THPVariable_Unpack(grad_h.ptr()).sizes();
+  const at::DimVector wide = Wide(of.slice(0, of.size() - 1)), index_wide = Wide(index.sizes());
+  if (n && wide.size() > 1 && index_wide.size() > 1 && wide != index_wide)
+    throw py::value_error("grad must be shaped [*index.shape, dim] or [indices, dim]");
   if (num_rows < 0 || num_rows >= (int64_t)1 << 31 || n >= (int64_t)1 << 31)
     throw py::value_error(std::to_string(n) + " indices into " + std::to_string(num_rows) + " rows: both must be below 2^31");
   const On on(grad.t);
