@@ -8,6 +8,9 @@
 //                                       mix <row bytes> <rows> <words>
 //                                       pool <id bytes> <row bytes> <ids> <samples> <max norm> <words>
 //                                       lists <bits>                                  one out of a bitmap, two out of two
+//                                       dispatch <hint> <tokens> <elements>           two fp32 rows a token; under an output hint
+//                                       take <hint> <rows> <elements>
+//                                       clip <hint> <elements>                        into another tensor
 // words: 0: nobody polls, 1: words are asked for (ugk_leave_done_words), 2: where they are faster, 3: and a key with them.
 // Prints a line per launch, the kernel, its template arguments, the stream, workgroups x threads and the other arguments, and how
 // many words the call says it leaves.
@@ -167,6 +170,20 @@ int main(int argc, char **argv) {
     const auto fn = reinterpret_cast<decltype(&ugk_extract_mix_i64)>(dlsym(lib, "ugk_extract_mix_i64"));
     rc = fn(flat, static_cast<int64_t *>(dev(2)), number(4), dev(1), 1000, dev(5), 1000, dev(3), number(3), u32, nullptr, nullptr,
             nullptr, UGK_HINT_UNKNOWN, dev(11));
+  } else if (call == "dispatch" || call == "take" || call == "clip") {
+    if (reinterpret_cast<decltype(&ugk_set_output_hint)>(dlsym(lib, "ugk_set_output_hint"))((int)number(3)) != 0) return 1;
+    int32_t *i32 = static_cast<int32_t *>(dev(2));
+    if (call == "dispatch") {
+      const auto fn = reinterpret_cast<decltype(&ugk_expert_dispatch)>(dlsym(lib, "ugk_expert_dispatch"));
+      rc = fn(dev(1), number(5), i32, static_cast<int32_t *>(dev(4)), number(4), 2, number(5), 4, dev(3), dev(11));
+    } else if (call == "take") {
+      const auto fn = reinterpret_cast<decltype(&ugk_take_rows_i32)>(dlsym(lib, "ugk_take_rows_i32"));
+      rc = fn(dev(1), 1000, number(5), i32, number(4), number(5), 4, dev(3), dev(11));
+    } else {
+      const ugk_tensor_t one{dev(1), dev(3), number(4), 4, 0};
+      const auto fn = reinterpret_cast<decltype(&ugk_grad_clip)>(dlsym(lib, "ugk_grad_clip"));
+      rc = fn(&one, 1, 1.0, dev(7), ~(size_t)0, static_cast<float *>(dev(5)), dev(11));
+    }
   } else if (call == "pool" && argc == 9 && ask(number(8))) {
     ugk_table_t none{};
     const auto run = [&](auto fn, auto *ids) {

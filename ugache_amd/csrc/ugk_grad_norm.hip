@@ -298,7 +298,7 @@ int ugk_grad_clip(const ugk_tensor_t *tensors, size_t n, double max_norm, void *
     read += tensors[i].count * elem_size(tensors[i].elem);
     if (tensors[i].out && tensors[i].out != tensors[i].data) written += tensors[i].count * elem_size(tensors[i].elem);
   }
-  const bool stream_out = nt_store_for(read + written);
+  const bool stream_out = read + written > kMemorySideCacheBytes;
   return for_lists(tensors, n, true, [&](const TensorList &list, uint64_t before) -> int {
     const uint32_t kept = before < kKept ? (uint32_t)(kKept - before) : 0;
     if (stream_out)

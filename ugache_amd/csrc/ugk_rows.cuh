@@ -118,11 +118,11 @@ static inline int for_rows_streamed(int elem, size_t dim, size_t rows, F f) {
 }
 // ... for kernels that move elements of two or four bytes without looking at them, and whether their output of so many rows is
 // stored past the caches (49,152 rows of 4 KB, 201 MB, past the caches / the ordinary way 40 / 36 us; 131,072, and their gradient
-// behind them, 224 / 259)
+// behind them, 224 / 259).  By size alone: what ugk_set_output_hint says is about the extractions of the thread.
 template <typename F>
 static inline int for_moved_rows(int elem, size_t dim, size_t out_rows, F f) {
   const auto stored = [&](auto type, auto vec) -> int {
-    return nt_store_for(out_rows * dim * sizeof(type)) ? f(type, vec, std::true_type()) : f(type, vec, std::false_type());
+    return out_rows * dim * sizeof(type) > kMemorySideCacheBytes ? f(type, vec, std::true_type()) : f(type, vec, std::false_type());
   };
   if (elem == 4) return dim >= 4 ? stored(uint32_t(), std::integral_constant<int, 4>()) : stored(uint32_t(), std::integral_constant<int, 1>());
   return dim >= 8 ? stored(uint16_t(), std::integral_constant<int, 8>()) : stored(uint16_t(), std::integral_constant<int, 1>());
