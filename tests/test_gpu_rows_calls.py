@@ -182,3 +182,80 @@ def test_a_gradient_in_another_order_than_its_index_is_refused():
     one = co.coll_torch_take_rows_grad(grad[0, 0], index[0, 0], 9)
     assert torch.equal(one[index[0, 0]], grad[0, 0]) and int(one.any(1).sum()) == int(grad[0, 0].any())
     assert not co.coll_torch_take_rows_grad(grad[:0], index.t()[:, :0], 9).any()
+
+
+# ---- between a forward and a backward pass ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("asks", ["rows, no weights", "rows", "weights", "both"])
+def test_what_no_gradient_reads_may_change_before_the_backward_pass(asks):
+    """the gradient of the rows reads the weights, that of the weights the rows, and neither its own"""
+    g = gen(6)
+    tokens, top, dim = 40, 3, 20
+    order = order_of(g, tokens, top, 8)
+    leaf, w = whole(g, tokens * top, dim), whole(g, tokens, top)
+    grad = whole(g, tokens, dim)
+    want_rows, want_w = co.coll_torch_expert_combine_grad(grad, leaf + 1, order, w)
+    if asks == "rows, no weights":
+        want_rows = co.coll_torch_expert_combine_grad(grad, leaf + 1, order)[0]
+    for changed in ("nothing", "rows", "weights"):
+        r = leaf.clone().requires_grad_(asks != "weights")
+        v = None if asks == "rows, no weights" else w.clone().requires_grad_(asks != "rows")
+        rows, weights = r + 1, None if v is None else v + 0  # made, not leaves: they may be changed in place
+        out = co.coll_torch_expert_combine(rows, order, weights)
+        with torch.no_grad():
+            if changed == "rows":
+                rows.mul_(5)
+            elif changed == "weights" and weights is not None:
+                weights.mul_(5)
+        if (changed == "rows" and asks in ("weights", "both")) or (changed == "weights" and asks in ("rows", "both")):
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                out.backward(grad)
+            continue
+        out.backward(grad)
+        assert r.grad is None if asks == "weights" else torch.equal(r.grad, want_rows)
+        if v is not None:
+            assert v.grad is None if asks == "rows" else torch.equal(v.grad, want_w)
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+def test_rows_that_no_gradient_reads_are_let_go(weighted):
+    g = gen(7)
+    order = order_of(g, 1000, 4, 8)
+    leaf = randn(g, 4000, 1024).requires_grad_()
+    w = torch.rand(1000, 4, device="cuda", generator=g) if weighted else None
+    out = co.coll_torch_expert_combine(leaf + 1, order, w)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    rows = leaf + 1
+    held = torch.cuda.memory_allocated() - before
+    assert held >= 4000 * 1024 * 4
+    again = co.coll_torch_expert_combine(rows, order, w)
+    del rows
+    assert torch.cuda.memory_allocated() - before < held  # the output is a quarter of the rows
+    assert torch.equal(torch.autograd.grad(out.sum(), leaf)[0], torch.autograd.grad(again.sum(), leaf)[0])
+
+
+def test_gradients_asked_for_one_at_a_time():
+    g = gen(8)
+    order = order_of(g, 50, 2, 8)
+    rows, w = whole(g, 100, 12).requires_grad_(), whole(g, 50, 2).requires_grad_()
+    grad = whole(g, 50, 12)
+    want = co.coll_torch_expert_combine_grad(grad, rows.detach(), order, w.detach())
+    for k, leaf in enumerate((rows, w)):
+        assert torch.equal(torch.autograd.grad(co.coll_torch_expert_combine(rows, order, w), leaf, grad)[0], want[k])
+    out = co.coll_torch_expert_combine(rows.view(50, 2, 12), order, w.half())
+    out.backward(grad)
+    assert torch.equal(rows.grad, want[0]) and torch.equal(w.grad, want[1])
+    none = torch.empty(0, 4, dtype=torch.int64, device="cuda")
+    nobody = torch.empty(0, 12, device="cuda").requires_grad_()
+    co.coll_torch_expert_combine(nobody, co.coll_torch_expert_sort(none, 8)).sum().backward()
+    assert nobody.grad.shape == (0, 12)
+
+
+def test_rows_are_left_out_only_where_nothing_reads_them():
+    g = gen(9)
+    order = order_of(g, 10, 2, 4)
+    for weights in (None, torch.rand(10, 2, device="cuda", generator=g)):
+        with pytest.raises(TypeError, match="rows"):
+            co.coll_torch_expert_combine_grad(randn(g, 10, 8), None, order, weights)

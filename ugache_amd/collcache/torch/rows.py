@@ -66,15 +66,20 @@ class _Dispatch(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, slot, offsets):
-        ctx.save_for_backward(rows, weights, slot, offsets)
+        # each gradient reads the other's values; those that no gradient reads may change, or go
+        for_rows, for_weights = ctx.needs_input_grad[:2]
+        ctx.save_for_backward(rows if for_weights else None, weights if for_rows else None, slot, offsets)
+        ctx.shape = rows.shape
+        ctx.unread = None if for_rows or weights is None else weights.detach()  # its shape and type
         return _native.combine(rows, slot, offsets, weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         rows, weights, slot, offsets = ctx.saved_tensors
-        grad_rows, grad_weights = _native.combine_grad(grad, rows, slot, offsets, weights, ctx.needs_input_grad[1])
-        return grad_rows.view(rows.shape), grad_weights, None, None
+        for_rows, for_weights = ctx.needs_input_grad[:2]
+        grad_rows, grad_weights = _native.combine_grad(grad, rows, slot, offsets, ctx.unread if weights is None else weights, for_weights)
+        return grad_rows.view(ctx.shape) if for_rows else None, grad_weights, None, None
 
 
 class _TakeRows(torch.autograd.Function):

@@ -202,23 +202,26 @@ py::object Combine(const char *what, py::handle rows_h, py::handle slot_h, py::h
   return Wrap(std::move(out));
 }
 
+// rows_h None: only where the gradient of the weights is not wanted (weights_too false), which alone reads the rows
 py::tuple CombineGrad(py::handle grad_h, py::handle rows_h, py::handle slot_h, py::handle offsets_h, py::handle weights_h,
                       bool weights_too) {
   const Rows grad = RowsOf("grad_out", grad_h);
   const int dev = grad.t.get_device();
-  const Rows rows = RowsOf("rows", rows_h, dev);
+  Rows rows{Tensor(), 0, grad.dim, grad.dim, grad.elem};
+  const bool read = weights_too || !rows_h.is_none();
+  if (read) rows = RowsOf("rows", rows_h, dev);
   const Order o = OrderOf(slot_h, offsets_h, dev);
-  if (grad.n != o.tokens || rows.n != o.n || grad.dim != rows.dim || grad.elem != rows.elem)
+  if (grad.n != o.tokens || (read && rows.n != o.n) || grad.dim != rows.dim || grad.elem != rows.elem)
     throw py::value_error("grad_out and rows are not rows of one type and length of " + std::to_string(o.tokens) + " tokens and " +
                           std::to_string(o.n) + " assignments");
   const Weights w = WeightsOf(weights_h, o, dev);
-  const On on(rows.t);
-  Tensor grad_rows = NewRows(o.n, rows);
+  const On on(grad.t);
+  Tensor grad_rows = NewRows(o.n, grad);
   Tensor grad_w;
   if (w.data && weights_too) grad_w = at::empty(w.t.sizes(), w.t.options());
   else if (w.t.defined() && weights_too) grad_w = at::empty_like(w.t);  // no assignments
-  Launched(ugk_expert_combine_grad(grad.t.data_ptr(), (size_t)grad.stride, rows.t.data_ptr(), (size_t)rows.stride, o.slot.data_ptr<int32_t>(),
-                                   o.live, (size_t)o.tokens, (uint32_t)o.top, w.data, w.elem, (size_t)rows.dim, rows.elem,
+  Launched(ugk_expert_combine_grad(grad.t.data_ptr(), (size_t)grad.stride, Data(rows.t), (size_t)rows.stride, o.slot.data_ptr<int32_t>(),
+                                   o.live, (size_t)o.tokens, (uint32_t)o.top, w.data, w.elem, (size_t)grad.dim, grad.elem,
                                    grad_rows.data_ptr(), Data(grad_w), on.stream));
   return py::make_tuple(Wrap(std::move(grad_rows)), grad_w.defined() ? Wrap(std::move(grad_w)) : py::none());
 }
