@@ -1,5 +1,6 @@
 """CPU tests of the calls of the operators on rows (collcache.torch) that are turned down, or answered, before any GPU is asked."""
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -97,3 +98,34 @@ def test_the_package_without_the_compiled_module(tmp_path, module):
         (copy / "collcache" / "torch" / os.path.basename(build.native_rows_path())).write_bytes(b"")
     done = subprocess.run([sys.executable, "-c", WITHOUT, str(copy)], cwd=tmp_path, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "went on" in done.stdout, done.stderr[-2000:]
+
+
+FOREIGN = """
+import importlib.util, sys
+import torch
+spec = importlib.util.spec_from_file_location("rows_native", sys.argv[1])
+module = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(module)
+print("loaded")
+"""
+
+
+@pytest.mark.parametrize("off,loads", [(0, True), (-1, False), (1, False)])
+def test_the_compiled_module_and_the_kernel_library_are_of_one_build(tmp_path, off, loads):
+    """beside a library of another ABI, whose calls take other arguments, the module is not loaded"""
+    native = build.native_rows_path()
+    called = [line.split()[-1] for line in subprocess.run(["nm", "-D", "--undefined-only", native], check=True, stdout=subprocess.PIPE,
+                                                          text=True).stdout.splitlines() if line.split()[-1].startswith("ugk_")]
+    version = int(re.search(r"#define UGK_ABI_VERSION (\d+)", open(os.path.join(build.INCLUDE, "ugache_hip.h")).read()).group(1))
+    (tmp_path / "stub.c").write_text("int ugk_abi_version(void) { return %d; }\n" % (version + off) + "".join(
+        "int %s(void) { return 1; }\n" % name for name in called if name != "ugk_abi_version"))
+    where = tmp_path / "ugache_amd" / "collcache" / "torch"
+    where.mkdir(parents=True)
+    subprocess.run(["gcc", "-shared", "-fPIC", str(tmp_path / "stub.c"), "-o", str(tmp_path / "ugache_amd" / "libugache_hip.so")], check=True)
+    shutil.copy(native, where)
+    done = subprocess.run([sys.executable, "-c", FOREIGN, str(where / os.path.basename(native))], cwd=tmp_path, capture_output=True, text=True,
+                          timeout=300)
+    if loads:
+        assert done.returncode == 0 and "loaded" in done.stdout, done.stderr[-2000:]
+    else:
+        assert done.returncode != 0 and "ImportError: libugache_hip.so and rows_native come from different builds" in done.stderr

@@ -399,6 +399,7 @@ py::object DispatchGrad(py::handle rows, py::handle slot, py::handle offsets) { 
 
 PYBIND11_MODULE(rows_native, m) {
   m.doc() = "the calls of collcache.torch.rows, compiled";
+  if (ugk_abi_version() != UGK_ABI_VERSION) throw py::import_error("libugache_hip.so and rows_native come from different builds");
   g_raw_stream = py::object(py::module_::import("torch._C").attr("_cuda_getCurrentRawStream")).release().ptr();
   g_launch_error = py::object(py::module_::import("builtins").attr("RuntimeError")).release().ptr();
   m.def("expert_sort", Guarded(&ExpertSort));
