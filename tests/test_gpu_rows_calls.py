@@ -259,3 +259,78 @@ def test_rows_are_left_out_only_where_nothing_reads_them():
     for weights in (None, torch.rand(10, 2, device="cuda", generator=g)):
         with pytest.raises(TypeError, match="rows"):
             co.coll_torch_expert_combine_grad(randn(g, 10, 8), None, order, weights)
+
+
+# ---- rows that very many entries name ---------------------------------------------------------------------------------
+
+# n entries over rows, each of `hot` rows named by its share of `share` of them.  Where rows are found by their position (rows > n,
+# or few short rows) and by themselves; more than 16 parts of a row, and of several rows in one workgroup; rows of one element, of
+# less than a chunk, and of more than 32 chunks, which are joined column by column
+HOT = [(30_000, 1, 24, 1, 1.0), (20_000, 2, 200, 2, 1.0), (700_000, 5, 12, 5, 1.0), (700_000, 5, 1, 2, 0.9), (120_000, 30_000, 48, 1, 0.999),
+       (120_000, 30_000, 48, 7, 0.7), (120_000, 300_000, 48, 1, 0.999), (120_000, 300_000, 3, 3, 0.8), (60_000, 70_000, 257, 1, 0.99),
+       (60_000, 20_000, 257, 3, 0.9), (60_000, 9000, 1030, 1, 0.95), (40_000, 50_000, 1030, 5, 0.5), (400_000, 3000, 9, 40, 0.95),
+       (1_200_000, 1_000_000, 4, 2, 0.6), (1_200_000, 2_000_000, 4, 300, 0.9), (4097, 5000, 300, 1, 1.0), (4000, 8000, 300, 1, 1.0)]
+
+
+def sums_of_whole(grad, index, rows):
+    """[rows, dim] float64: differences of running sums over the entries in order of their rows, exact in whole numbers"""
+    order = torch.sort(index).indices
+    upto = torch.cat([torch.zeros(1, grad.size(1), dtype=torch.float64, device="cuda"), torch.cumsum(grad.double()[order], 0)])
+    ends = torch.cumsum(torch.bincount(index, minlength=rows), 0)
+    return upto[ends] - torch.cat([upto[:1], upto[ends[:-1]]])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,rows,dim,hot,share", HOT)
+def test_no_entry_of_a_row_that_many_name_is_lost(n, rows, dim, hot, share, dtype):
+    """whole numbers of at most 3 and fewer than 2^22 entries: every partial sum is exact in float32, so the result is the exact
+    sum rounded once, whatever the order"""
+    g = gen(n + rows + dim)
+    index = torch.randint(0, rows, (n,), device="cuda", generator=g)
+    named = torch.randperm(rows, device="cuda", generator=g)[torch.randint(0, hot, (n,), device="cuda", generator=g)]
+    index = torch.where(torch.rand(n, device="cuda", generator=g) < share, named, index)
+    grad = whole(g, n, dim, dtype=dtype)
+    assert torch.equal(co.coll_torch_take_rows_grad(grad, index, rows), sums_of_whole(grad, index, rows).to(dtype))
+    runs = torch.sort(index).values  # the same in order, so that the row's entries are neighbours before they are sorted too
+    assert torch.equal(co.coll_torch_take_rows_grad(grad, runs.int(), rows), sums_of_whole(grad, runs, rows).to(dtype))
+
+
+# ---- products and squares, none lost -----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [1, 7, 8, 9, 255, 257, 511, 1001, 1025, 2047, 2049, 4099, 17_001])
+def test_no_product_of_a_long_row_is_lost(dim, dtype):
+    """dots of whole numbers of at most 3: every partial sum is below 2^24 and exact, also where chunks of a row overlap"""
+    g = gen(dim)
+    tokens, top = 19, 5
+    order = order_of(g, tokens, top, 8)
+    rows, grad, w = whole(g, tokens * top, dim, dtype=dtype), whole(g, tokens, dim, dtype=dtype), whole(g, tokens, top)
+    grad_rows, grad_w = co.coll_torch_expert_combine_grad(grad, rows, order, w)
+    at = rows[order.slot.long()].double()
+    assert torch.equal(grad_w.double(), (at * grad.double().unsqueeze(1)).sum(-1))
+    assert torch.equal(grad_rows[order.slot.long()].double(), grad.double().unsqueeze(1) * w.double().unsqueeze(-1))
+    assert torch.equal(co.coll_torch_expert_combine(rows, order, w).double(), (at * w.double().unsqueeze(-1)).sum(1))
+
+
+@pytest.mark.parametrize("sizes", [(1, 8191, 8192, 8193, 16_385), (100_000_003, 60_000_001, 5)])
+def test_no_square_is_lost(sizes):
+    """tensors of zeros with threes at their ends, at the ends of the pieces that are summed, and anywhere: a norm is the root of
+    nine times their number, rounded once"""
+    g = gen(len(sizes))
+    grads = [torch.zeros(n, device="cuda", dtype=torch.bfloat16 if k % 2 == 0 else torch.float32) for k, n in enumerate(sizes)]
+    for turn in range(6):
+        count = 0
+        for t in grads:
+            n, piece = t.numel(), 32_768 // t.element_size()
+            at = torch.randint(0, n, (3,), device="cuda", generator=g)
+            if turn < 3:
+                k = int(torch.randint(0, n // piece + 1, (1,), device="cuda", generator=g))
+                at = torch.tensor([0, n - 1, k * piece - 1, k * piece, n // 8 * 8 - 1], device="cuda").clamp(0, n - 1)
+            t.zero_()[at] = 3
+            count += torch.unique(at).numel()
+        norm = torch.tensor(9.0 * count, dtype=torch.float64).sqrt().float()
+        assert torch.equal(co.coll_torch_grad_norm(grads).cpu(), norm)
+        out = [torch.empty_like(t) for t in grads]
+        assert torch.equal(co.coll_torch_clip_grad_norm(grads, 1e9, out=out).cpu(), norm)
+        assert all(torch.equal(a, b) for a, b in zip(out, grads))
