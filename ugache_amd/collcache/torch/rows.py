@@ -4,8 +4,8 @@ the reference looks rows up and trains none).
 Torch operators over the kernels of include/ugache_hip.h: GPU tensors of float32, float16 or bfloat16 in and out, enqueued
 on torch's current stream of the tensors' device like any torch op, no host wait, no atomics in a sum: the same
 inputs give the same bits.  Every call takes its memory from torch, so calls on several streams and calls recorded into
-HIP graphs share nothing.  What cannot be computed raises TypeError or ValueError before anything is enqueued; a failing
-launch raises RuntimeError.
+HIP graphs share nothing.  Bad arguments raise TypeError or ValueError before anything is enqueued; sizes beyond what one launch
+takes, and a launch that fails, raise RuntimeError.  Rows whose elements are not neighbours (a transposed table) are copied first.
 
 The operators that are called differentiable below record their gradient (torch.autograd, reverse mode) where an input asks
 for one; the gradients are entry points of their own as well, for programs that call backward passes themselves, and record

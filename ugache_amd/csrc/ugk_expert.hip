@@ -260,8 +260,10 @@ int ugk_expert_combine_grad(const void *grad_out_dev, size_t grad_stride, const 
     const uint32_t chunks = split_of(dim, V).chunks;
     uint32_t lanes = 4;
     while (lanes < chunks && lanes < (uint32_t)kWave) lanes *= 2;
-    // a workgroup per token from 256 chunks on (us, both gradients of K rows of a token and the sum: 16,384 x 8 x 256 chunks 317
-    // against 335 with a wavefront per token; 4,099 x 3 x 251 chunks 33.5 against 32.4, 4,096 x 8 x 128 chunks 49 against 40)
+    // a workgroup per token from 256 chunks on (us, a wavefront / a workgroup per token, bfloat16 rows: 1 GB of them, eight a token, of
+    // 128 chunks 396 / 492, 192 408 / 399, 256 410 / 391, 512 459 / 411, 1,024 453 / 422; 16 MB, eight a token, 256 16.5 / 12.1; two a
+    // token, where fewer rows are on their way in a workgroup, change over later: 1 GB, 256 477 / 541, 320 485 / 495, 512 535 / 465;
+    // 16 MB, 256 10.1 / 12.7, 512 11.7 / 10.1)
     const bool wide = chunks >= (uint32_t)kBlock;
     const auto launch = [&](auto is_wide, size_t blocks, uint32_t of) -> int {
       hipLaunchKernelGGL((combine_grad_kernel<T, V, S, decltype(is_wide)::value>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),

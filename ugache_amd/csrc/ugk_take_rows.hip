@@ -291,6 +291,8 @@ int take_rows(const void *table, uint64_t num_rows, size_t stride, const I *inde
 }
 
 // how a batch of n entries over `rows` rows is sorted: digits of equal length, the key `rows` (no row) among them
+// (as few digits as ten bits allow; us of the gradient of rows of 32 bytes by position over 2^20 - 1 rows, two digits of ten bits,
+// and over 2^20 + 1, three of seven: 250,000 entries 52.5 and 50.4, 500,000 67.3 and 63.0, 1,000,000 91.2 and 84.5)
 struct Plan {
   uint32_t passes, digit;
 };
@@ -306,7 +308,10 @@ Plan plan_for(uint64_t rows) {
 // 16,384 entries over 50,000 bfloat16 rows of 2 KB 46 / 62, 40,000 over 50,000 76 / 98, 100,000 over 200,000 of 256 bytes 70 / 69;
 // 3,000 over 3,000 of 128 bytes 18.6 / 21.0, 10,000 over 5,000 of 256 bytes 30 / 31, 213,119 over as many of 16 bytes 37 / 42;
 // 40,000 over 40,000 of 4 KB 145 / 111, 262,144 over 60,000 of 512 bytes 133 / 105, 100,000 over 2,000 of 1 KB 59 / 48, 928,382 over
-// 42,603 of 8 bytes 84 / 70.
+// 42,603 of 8 bytes 84 / 70.  The line of 4,000,000 elements is between the types' own, which lie near 12 MB of output (fp32
+// rows of 400 bytes 2.8 M elements 34.6 / 32.5, 3.8 M 39.4 / 35.4; bfloat16 rows of 1,000 bytes 4.2 M 25.7 / 26.5, 5.6 M 28.1 / 29.4,
+// 8.4 M 37.1 / 34.4).  Rows that outnumber the entries a little are visited by position too, which costs where they are many MB:
+// 285,714 bfloat16 rows of 2 KB and 200,000 entries 392 / 281, of 16 bytes 42.6 / 47.3.
 bool sums_by_row(size_t n, uint64_t rows, size_t dim) { return rows <= n && (rows * dim > 4'000'000 || (n > 32768 && n > 2 * rows)); }
 
 // Entries a lane adds one after the other: few where the batch is small and their latency is what it costs, more where the
